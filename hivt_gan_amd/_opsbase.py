@@ -44,6 +44,14 @@ def _need_gpu(*tensors: torch.Tensor) -> None:
                                "there is no CPU fallback in the product path")
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(t: torch.Tensor):
+    """Makes ``t``'s device the current one for the calls inside (a launch goes to the current device)."""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def _workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 

@@ -1,0 +1,624 @@
+// Backward of the attention with a learned bias for each bucket of relative positions.
+//
+// No atomics, so equal calls give equal bits.  Three passes recompute the weights from the saved statistics:
+//   dq_kernel    a workgroup owns query rows and walks the keys: dq, and what each row's ds sum up to;
+//   dkv_kernel   a workgroup owns keys and walks the query rows of every head of the group: dk, dv;
+//   bias_kernel  a wave owns query rows and walks the keys nearer than the last bucket: sums of ds along diagonals.
+//
+// The bias gradient needs more care than the others.  Each row of ds sums to zero, so a bucket that holds most keys of
+// most rows is left with the small rest of that cancellation, and an error of delta_i (it comes from an output that is
+// rounded, and whose weights were rounded for the matrix cores) enters it once per row, all with one sign for a row.
+// dq_kernel therefore adds up r_i = sum_j ds_ij in fp32, which is that error (the weights of a row sum to one), writes
+// delta_i + r_i for the passes behind it, and corrects its own sums over the far keys by r_i times their weights.
+#include "relative_core.h"
+
+namespace hivt {
+namespace rel {
+namespace {
+
+constexpr int kBN = 64;
+
+// d_out . out of a lane's share of a row
+template <typename T, int E>
+__device__ __forceinline__ float dot(const Frag<T, E>& a, const Frag<T, E>& b) {
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < E; ++j) s = fmaf((float)a.v[j], (float)b.v[j], s);
+  return s;
+}
+
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restrict__ far_sums) {
+  using TL = Tile<T, DP>;
+  constexpr int NB = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const kt = reinterpret_cast<T*>(smem);
+  T* const vt = kt + kBN * TL::PITCH;
+  float* const bias = reinterpret_cast<float*>(vt + kBN * TL::PITCH);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4;
+  const int qtiles = (a.M + 64 * QB - 1) / (64 * QB);
+  int unit, inner;
+  walk(blockIdx.x, a.B * a.H, qtiles, unit, inner);
+  const int qtile = qtiles - 1 - inner;
+  const int b = unit / a.H, h = unit % a.H, g = h / a.rep;
+  const int width = bias_width(a), hi = bias_hi(a);
+  for (int e = tid; e < width; e += 256) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+
+  const int row0 = qtile * 64 * QB + wave * 16 * QB;
+  const bool active = row0 < a.M;
+  int pos[QB];
+  bool live[QB];
+  float m[QB], il[QB], delta[QB], rsum[QB];
+  Frag<T, TL::E> qf[QB][TL::KSTEPS], of[QB][TL::KSTEPS];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = row0 + qb * 16 + (lane & 15);
+    live[qb] = r < a.M;
+    const int s = min(r, a.M - 1);
+    pos[qb] = s + a.offset;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_st[0] + s * a.q_st[1] + h * a.q_st[2];
+    const T* go = static_cast<const T*>(a.d_out) + b * a.do_st[0] + s * a.do_st[1] + h * a.do_st[2];
+    const T* out = static_cast<const T*>(a.out) + b * a.o_st[0] + s * a.o_st[1] + h * a.o_st[2];
+    float part = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+      const int col = ks * TL::KS + quad * TL::E;
+      qf[qb][ks] = load_frag<T, TL::E>(q, col, a.d, a.q_align, live[qb]);
+      of[qb][ks] = load_frag<T, TL::E>(go, col, a.d, a.do_align, live[qb]);
+      part += dot(of[qb][ks], load_frag<T, TL::E>(out, col, a.d, a.o_align, live[qb]));
+    }
+    delta[qb] = quad_sum(part);
+    const float2 st = live[qb] ? a.stats[((int64_t)b * a.H + h) * a.M + s] : make_float2(0.0f, 0.0f);
+    m[qb] = st.x;
+    il[qb] = st.y;
+    rsum[qb] = 0.0f;
+  }
+  const int pos_lo = min(row0, a.M - 1) + a.offset, pos_hi = max(min(row0 + 16 * QB, a.M) - 1, 0) + a.offset;
+  const int wg_last = min((qtile + 1) * 64 * QB, a.M) - 1 + a.offset;
+  const int keys_end = a.causal ? min(a.N, wg_last + 1) : a.N;
+  const int t_end = keys_end > 0 ? (keys_end + kBN - 1) / kBN : 0;
+
+  f32x4 dq[NB][QB];
+  float far_l[QB], far_r[QB], w_l[QB], w_r[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    far_l[qb] = far_r[qb] = w_l[qb] = w_r[qb] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) dq[n][qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const T* const kbase = static_cast<const T*>(a.k) + b * a.k_st[0] + g * a.k_st[2];
+  const T* const vbase = static_cast<const T*>(a.v) + b * a.v_st[0] + g * a.v_st[2];
+  Loader<T, DP, kBN, 256> kl, vl;
+  uint64_t bits = 0;
+  int t = 0;
+  auto seek = [&]() {
+    while (t < t_end && (bits = tile_keys(a, b, t * kBN, lane)) == 0) ++t;
+    if (t < t_end) {
+      const int64_t k0 = (int64_t)t * kBN;
+      auto keep = [&](int row) { return (bits >> row & 1) != 0; };
+      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, keep);
+      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, keep);
+    }
+  };
+  seek();
+  while (t < t_end) {
+    __syncthreads();
+    kl.store(kt, tid);
+    vl.store(vt, tid);
+    const int k0 = t * kBN;
+    const uint64_t keys = bits;
+    ++t;
+    seek();
+    __syncthreads();
+    if (!active || (a.causal && k0 > pos_hi)) continue;
+
+    const int rel_hi = k0 + kBN - 1 - pos_lo, rel_lo = k0 - pos_hi;
+    const bool left = rel_hi <= -a.sat, right = rel_lo >= hi, far = left || right;
+    const bool whole = keys == ~0ull && (!a.causal || rel_hi <= 0);
+    // two 16-key blocks at a time: what the reduction over the keys takes
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      f32x4 s[2][QB], dp[2][QB];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) s[i][qb] = dp[i][qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+          const Frag<T, TL::E> kf = TL::rows(kt, (2 * kk + i) * 16, ks, lane), vf = TL::rows(vt, (2 * kk + i) * 16, ks, lane);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) {
+            Frag<T, TL::E>::mma(kf, qf[qb][ks], s[i][qb]);
+            Frag<T, TL::E>::mma(vf, of[qb][ks], dp[i][qb]);
+          }
+        }
+      }
+      Frag<T, 8> df[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const int rel0 = k0 + kk * 32 + quad * 4 - pos[qb] + a.sat;
+        const int lim = a.causal ? pos[qb] - k0 : kBN;
+        const float c = bias[left ? 0 : width - 1];
+        float sum_ds = 0.0f, sum_p = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float add = far ? c : bias[min(max(rel0 + i * 16 + r, 0), width - 1)];
+            float p = fexp2(fmaf(s[i][qb][r], a.scale2, add) - m[qb]) * il[qb];
+            if (!whole && (!(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim)) p = dp[i][qb][r] = 0.0f;
+            const float ds = p * (dp[i][qb][r] - delta[qb]);
+            dp[i][qb][r] = ds;
+            sum_ds += ds;
+            sum_p += p;
+          }
+        }
+        rsum[qb] += sum_ds;
+        if (left) { far_l[qb] += sum_ds; w_l[qb] += sum_p; }
+        else if (right) { far_r[qb] += sum_ds; w_r[qb] += sum_p; }
+        df[qb] = pair_frag<T>(dp[0][qb], dp[1][qb]);
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const Frag<T, 8> kf = TL::cols(kt, kk * 32, n * 16, lane);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) Frag<T, 8>::mma(kf, df[qb], dq[n][qb]);
+      }
+    }
+  }
+  if (!active) return;
+
+  float sum_l = 0.0f, sum_r = 0.0f;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const float r = quad_sum(rsum[qb]);
+    sum_l += quad_sum(far_l[qb]) - r * quad_sum(w_l[qb]);
+    sum_r += quad_sum(far_r[qb]) - r * quad_sum(w_r[qb]);
+    if (!live[qb]) continue;
+    const int s = row0 + qb * 16 + (lane & 15);
+    if (quad == 0) a.delta[((int64_t)b * a.H + h) * a.M + s] = delta[qb] + r;
+    T* out = static_cast<T*>(a.dq) + b * a.dq_st[0] + s * a.dq_st[1] + h * a.dq_st[2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      f32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = dq[n][qb][j] * a.scale;
+      store4(out, n * 16 + quad * 4, a.d, w);
+    }
+  }
+  if (far_sums != nullptr) {
+    sum_l = group_sum<16>(sum_l);
+    sum_r = group_sum<16>(sum_r);
+    const int groups = (a.M + 16 * QB - 1) / (16 * QB);
+    if (lane == 0) far_sums[(int64_t)unit * groups + row0 / (16 * QB)] = make_float2(sum_l, sum_r);
+  }
+}
+
+// BQ query rows a step; a wave owns 16 KB keys.
+template <typename T, int DP, int KB, int BQ>
+__global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int NB = DP / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const qt = reinterpret_cast<T*>(smem);
+  T* const ot = qt + BQ * TL::PITCH;
+  float4* const rowst = reinterpret_cast<float4*>(ot + BQ * TL::PITCH);  // m, 1 / l, delta of a row
+  float* const bias = reinterpret_cast<float*>(rowst + BQ);
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4;
+  const int ktiles = (a.N + 64 * KB - 1) / (64 * KB);
+  int unit, ktile;
+  walk(blockIdx.x, a.B * a.G, ktiles, unit, ktile);
+  const int b = unit / a.G, g = unit % a.G;
+  const int width = bias_width(a), hi = bias_hi(a);
+
+  const int key0 = ktile * 64 * KB + wave * 16 * KB;
+  bool keep[KB];
+  int key[KB];
+  Frag<T, TL::E> kf[KB][TL::KSTEPS], vf[KB][TL::KSTEPS];
+  bool any = false;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    key[kb] = key0 + kb * 16 + (lane & 15);
+    keep[kb] = key[kb] < a.N && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_sb + key[kb]] == 0);
+    any = any || keep[kb];
+    const int64_t kc = min(key[kb], a.N - 1);
+    const T* k = static_cast<const T*>(a.k) + b * a.k_st[0] + kc * a.k_st[1] + g * a.k_st[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.v_st[0] + kc * a.v_st[1] + g * a.v_st[2];
+#pragma unroll
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+      const int col = ks * TL::KS + quad * TL::E;
+      kf[kb][ks] = load_frag<T, TL::E>(k, col, a.d, a.k_align, keep[kb]);
+      vf[kb][ks] = load_frag<T, TL::E>(v, col, a.d, a.v_align, keep[kb]);
+    }
+  }
+  const bool active = __any(any);
+  const bool all = __all([&]() { bool x = true;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) x = x && keep[kb];
+    return x; }());
+  const int key_hi = min(key0 + 16 * KB, a.N) - 1;
+
+  f32x4 dk[NB][KB], dv[NB][KB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) dk[n][kb] = dv[n][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int qsteps = (a.M + BQ - 1) / BQ;
+  const int first = a.causal ? max(0, ktile * 64 * KB - a.offset) / BQ : 0;  // rows before it see none of these keys
+  Loader<T, DP, BQ, 256> ql, ol;
+  for (int hr = 0; hr < a.rep; ++hr) {
+    const int h = g * a.rep + hr;
+    __syncthreads();  // the head before has been finished by every wave
+    for (int e = tid; e < width; e += 256) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+    const T* const qbase = static_cast<const T*>(a.q) + b * a.q_st[0] + h * a.q_st[2];
+    const T* const obase = static_cast<const T*>(a.d_out) + b * a.do_st[0] + h * a.do_st[2];
+    const int64_t rowbase = ((int64_t)b * a.H + h) * a.M;
+    float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto fetch = [&](int step) {
+      const int s0 = step * BQ;
+      auto in = [&](int row) { return s0 + row < a.M; };
+      ql.load(qbase + (int64_t)s0 * a.q_st[1], a.q_st[1], a.d, a.q_align, tid, in);
+      ol.load(obase + (int64_t)s0 * a.do_st[1], a.do_st[1], a.d, a.do_align, tid, in);
+      if (tid < BQ) {
+        st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (s0 + tid < a.M) {
+          const float2 s2 = a.stats[rowbase + s0 + tid];
+          st = make_float4(s2.x, s2.y, a.delta[rowbase + s0 + tid], 0.0f);
+        }
+      }
+    };
+    if (first < qsteps) fetch(first);
+    for (int step = first; step < qsteps; ++step) {
+      __syncthreads();
+      ql.store(qt, tid);
+      ol.store(ot, tid);
+      if (tid < BQ) rowst[tid] = st;
+      if (step + 1 < qsteps) fetch(step + 1);
+      __syncthreads();
+      const int s0 = step * BQ, pos0 = s0 + a.offset;
+      const int pos_last = min(s0 + BQ, a.M) - 1 + a.offset;
+      if (!active || (a.causal && key0 > pos_last)) continue;
+      const int rel_hi = key_hi - pos0, rel_lo = key0 - pos_last;
+      const bool left = rel_hi <= -a.sat, far = left || rel_lo >= hi;
+      const bool whole = all && s0 + BQ <= a.M && (!a.causal || rel_hi <= 0);
+      const float c = bias[left ? 0 : width - 1];
+#pragma unroll
+      for (int qq = 0; qq < BQ / 32; ++qq) {
+        f32x4 p[2][KB], ds[2][KB];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) p[i][kb] = ds[i][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+            const Frag<T, TL::E> qf = TL::rows(qt, qq * 32 + i * 16, ks, lane), of = TL::rows(ot, qq * 32 + i * 16, ks, lane);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+              Frag<T, TL::E>::mma(qf, kf[kb][ks], p[i][kb]);
+              Frag<T, TL::E>::mma(of, vf[kb][ks], ds[i][kb]);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = qq * 32 + i * 16 + quad * 4 + r;
+            const float4 rs = rowst[row];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+              const int rel = key[kb] - pos0 - row;
+              const float add = far ? c : bias[min(max(rel + a.sat, 0), width - 1)];
+              float w = fexp2(fmaf(p[i][kb][r], a.scale2, add) - rs.x) * rs.y;
+              float dp = ds[i][kb][r];
+              if (!whole && (!keep[kb] || s0 + row >= a.M || (a.causal && rel > 0))) w = dp = 0.0f;
+              p[i][kb][r] = w;
+              ds[i][kb][r] = w * (dp - rs.z);
+            }
+          }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const Frag<T, 8> pf = pair_frag<T>(p[0][kb], p[1][kb]), df = pair_frag<T>(ds[0][kb], ds[1][kb]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            Frag<T, 8>::mma(TL::cols(ot, qq * 32, n * 16, lane), pf, dv[n][kb]);
+            Frag<T, 8>::mma(TL::cols(qt, qq * 32, n * 16, lane), df, dk[n][kb]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    if (key[kb] >= a.N) continue;
+    T* ok = static_cast<T*>(a.dk) + b * a.dk_st[0] + key[kb] * a.dk_st[1] + g * a.dk_st[2];
+    T* ov = static_cast<T*>(a.dv) + b * a.dv_st[0] + key[kb] * a.dv_st[1] + g * a.dv_st[2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      f32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = keep[kb] ? dk[n][kb][j] * a.scale : 0.0f;
+      store4(ok, n * 16 + quad * 4, a.d, w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = keep[kb] ? dv[n][kb][j] : 0.0f;
+      store4(ov, n * 16 + quad * 4, a.d, w);
+    }
+  }
+}
+
+// Sums of ds over the buckets, for 16 QB query rows of one (batch, head): the tiles that dq_kernel did not count as far.
+// The tile of ds passes through LDS so that a lane can add along a diagonal; diagonals add up in LDS (one lane each, no
+// conflicts), distances beyond the last border in registers.
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __restrict__ far_sums,
+                                                  float* __restrict__ partial) {
+  using TL = Tile<T, DP>;
+  constexpr int ROWS = 16 * QB, PITCH = kBN + 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* const skew = reinterpret_cast<float*>(smem);
+  float* const bias = skew + ROWS * PITCH;
+  const int width = bias_width(a), hi = bias_hi(a);
+  float* const diag = bias + width;
+
+  const int lane = threadIdx.x, quad = lane >> 4;
+  const int groups = (a.M + ROWS - 1) / ROWS;
+  int unit, group;
+  walk(blockIdx.x, a.B * a.H, groups, unit, group);
+  const int b = unit / a.H, h = unit % a.H, g = h / a.rep;
+  for (int e = lane; e < width; e += 64) {
+    bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+    diag[e] = 0.0f;
+  }
+  __syncthreads();
+  const int row0 = group * ROWS;
+  int pos[QB];
+  float m[QB], il[QB], delta[QB];
+  Frag<T, TL::E> qf[QB][TL::KSTEPS], of[QB][TL::KSTEPS];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const int r = row0 + qb * 16 + (lane & 15);
+    const bool live = r < a.M;
+    const int s = min(r, a.M - 1);
+    pos[qb] = r + a.offset;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_st[0] + s * a.q_st[1] + h * a.q_st[2];
+    const T* go = static_cast<const T*>(a.d_out) + b * a.do_st[0] + s * a.do_st[1] + h * a.do_st[2];
+#pragma unroll
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+      qf[qb][ks] = load_frag<T, TL::E>(q, ks * TL::KS + quad * TL::E, a.d, a.q_align, live);
+      of[qb][ks] = load_frag<T, TL::E>(go, ks * TL::KS + quad * TL::E, a.d, a.do_align, live);
+    }
+    const int64_t at = ((int64_t)b * a.H + h) * a.M + s;
+    const float2 st = live ? a.stats[at] : make_float2(0.0f, 0.0f);
+    m[qb] = st.x;
+    il[qb] = st.y;
+    delta[qb] = live ? a.delta[at] : 0.0f;
+  }
+  const int pos_lo = row0 + a.offset, pos_hi = min(row0 + ROWS, a.M) - 1 + a.offset;
+  const int keys_end = a.causal ? min(a.N, pos_hi + 1) : a.N;
+  // the tiles that are not far: rel_hi > -sat and rel_lo < hi
+  const int t_begin = max(0, pos_lo - a.sat) / kBN;
+  const int t_end = min(keys_end > 0 ? (keys_end + kBN - 1) / kBN : 0, max(0, (pos_hi + hi + kBN - 1) / kBN + 1));
+  const T* const kbase = static_cast<const T*>(a.k) + b * a.k_st[0] + g * a.k_st[2];
+  const T* const vbase = static_cast<const T*>(a.v) + b * a.v_st[0] + g * a.v_st[2];
+  float acc_l = 0.0f, acc_r = 0.0f;
+  for (int t = t_begin; t < t_end; ++t) {
+    const int k0 = t * kBN;
+    const int rel_hi = k0 + kBN - 1 - pos_lo, rel_lo = k0 - pos_hi;
+    if (rel_hi <= -a.sat || rel_lo >= hi) continue;
+    const uint64_t keys = tile_keys(a, b, k0, lane);
+    if (keys == 0) continue;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      const int key = k0 + kb * 16 + (lane & 15);
+      const bool keep = (keys >> (kb * 16 + (lane & 15)) & 1) != 0;
+      const int64_t kc = min(key, a.N - 1);
+      f32x4 s[QB], dp[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) s[qb] = dp[qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+        const int col = ks * TL::KS + quad * TL::E;
+        const Frag<T, TL::E> kf = load_frag<T, TL::E>(kbase + kc * a.k_st[1], col, a.d, a.k_align, keep);
+        const Frag<T, TL::E> vf = load_frag<T, TL::E>(vbase + kc * a.v_st[1], col, a.d, a.v_align, keep);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          Frag<T, TL::E>::mma(kf, qf[qb][ks], s[qb]);
+          Frag<T, TL::E>::mma(vf, of[qb][ks], dp[qb]);
+        }
+      }
+      const uint32_t nibble = (uint32_t)(keys >> (kb * 16 + quad * 4));
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const int rel0 = k0 + kb * 16 + quad * 4 - pos[qb];
+        f32x4 ds;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float add = bias[min(max(rel0 + r + a.sat, 0), width - 1)];
+          const float p = fexp2(fmaf(s[qb][r], a.scale2, add) - m[qb]) * il[qb];
+          const bool out = !(nibble >> r & 1) || (a.causal && rel0 + r > 0) || pos[qb] > pos_hi;
+          ds[r] = out ? 0.0f : p * (dp[qb][r] - delta[qb]);
+        }
+        *reinterpret_cast<f32x4*>(skew + (qb * 16 + (lane & 15)) * PITCH + kb * 16 + quad * 4) = ds;
+      }
+    }
+    __syncthreads();
+    // diagonal c: key - row = c - (ROWS - 1) within the tile
+#pragma unroll
+    for (int c0 = 0; c0 < kBN + ROWS - 1; c0 += 64) {
+      const int c = c0 + lane;
+      const int rel = k0 - pos_lo + c - (ROWS - 1);
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int r = 0; r < ROWS; ++r) {
+        const int j = c - (ROWS - 1) + r;
+        if (j >= 0 && j < kBN) sum += skew[r * PITCH + j];
+      }
+      if (c < kBN + ROWS - 1) {
+        if (rel <= -a.sat) acc_l += sum;
+        else if (rel >= hi) acc_r += sum;
+        else diag[rel + a.sat] += sum;
+      }
+      __syncthreads();
+    }
+  }
+  const float2 fs = far_sums[(int64_t)unit * groups + group];
+  acc_l = wave_sum(acc_l) + fs.x;
+  acc_r = wave_sum(acc_r) + fs.y;
+  if (lane == 0) {
+    diag[0] += acc_l;
+    diag[width - 1] += acc_r;
+  }
+  __syncthreads();
+  const int side = a.bidirectional ? a.buckets / 2 : a.buckets;
+  for (int bucket = lane; bucket < a.buckets; bucket += 64) {
+    const bool behind = bucket >= side;  // keys behind the query
+    const int sb = behind ? bucket - side : bucket;
+    int from = sb < a.exact ? sb : sb == a.exact ? a.exact : a.starts[sb - a.exact - 1];
+    const int to = sb < a.exact ? sb + 1 : sb - a.exact < a.nstarts ? a.starts[sb - a.exact] : a.sat + 1;
+    if (behind && from == 0) from = 1;  // distance 0 belongs to the other side
+    float sum = 0.0f;
+    for (int n = from; n < to; ++n) sum += diag[behind ? a.sat + n : a.sat - n];
+    partial[((int64_t)unit * groups + group) * a.buckets + bucket] = sum;
+  }
+}
+
+// d_table[bucket][h] = the partial sums of head h, over batches and row groups in ascending order within each of the 16
+// slices a workgroup cuts them into, the slices in ascending order; in 64 bits.
+__global__ __launch_bounds__(1024) void table_kernel(const Args a, const float* __restrict__ partial, int groups,
+                                                     float* __restrict__ d_table) {
+  __shared__ double sums[16][64];
+  const int h = blockIdx.x, bucket = blockIdx.y * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+  const int64_t count = (int64_t)a.B * groups;
+  double s = 0.0;
+  if (bucket < a.buckets) {
+    const int64_t end = count * (slice + 1) / 16;
+    for (int64_t i = count * slice / 16; i < end; ++i) {
+      const int64_t b = i / groups, grp = i % groups;
+      s += partial[((b * a.H + h) * groups + grp) * a.buckets + bucket];
+    }
+  }
+  sums[slice][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (slice == 0 && bucket < a.buckets) {
+    for (int i = 1; i < 16; ++i) s += sums[i][threadIdx.x];
+    d_table[(int64_t)bucket * a.H + h] = (float)s;
+  }
+}
+
+constexpr int rows_per_group(int M) { return M <= 64 ? 16 : 32; }
+
+struct Work {
+  size_t delta, far, partial, total;
+  int groups;
+};
+Work work_of(const Args& a) {
+  Work w;
+  w.groups = (a.M + rows_per_group(a.M) - 1) / rows_per_group(a.M);
+  w.delta = 0;
+  w.far = align_up((size_t)a.B * a.H * a.M * sizeof(float), 256);
+  w.partial = w.far + (a.want_table ? align_up((size_t)a.B * a.H * w.groups * sizeof(float2), 256) : 0);
+  w.total = w.partial + (a.want_table ? align_up((size_t)a.B * a.H * w.groups * a.buckets * sizeof(float), 256) : 0);
+  return w;
+}
+
+template <typename T, int DP, int QB>
+int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
+  using TL = Tile<T, DP>;
+  const char* what = "hivt_relative_attn_bwd";
+  const size_t table = (size_t)bias_width(a) * sizeof(float);
+  float2* const far_sums = a.want_table ? reinterpret_cast<float2*>(ws + w.far) : nullptr;
+  const int64_t blocks = (int64_t)a.B * a.H * ((a.M + 64 * QB - 1) / (64 * QB));
+  const size_t lds = (size_t)2 * kBN * TL::PITCH * sizeof(T) + table;
+  HIVT_REQUIRE(blocks < ((int64_t)1 << 31) && (int64_t)a.B * a.H * w.groups < ((int64_t)1 << 31), HIVT_ERR_ARG,
+               "%s: too many workgroups", what);
+  if (lds > 48 * 1024)
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&dq_kernel<T, DP, QB>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
+  hipLaunchKernelGGL((dq_kernel<T, DP, QB>), dim3((unsigned)blocks), dim3(256), lds, stream, a, far_sums);
+  HIVT_CHECK_LAUNCH(what);
+  if (a.want_table) {
+    const size_t lb = (size_t)16 * QB * (kBN + 4) * sizeof(float) + 2 * table;
+    float* const partial = reinterpret_cast<float*>(ws + w.partial);
+    if (lb > 48 * 1024)
+      HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&bias_kernel<T, DP, QB>),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lb), what);
+    hipLaunchKernelGGL((bias_kernel<T, DP, QB>), dim3((unsigned)((int64_t)a.B * a.H * w.groups)), dim3(64), lb, stream, a,
+                       far_sums, partial);
+    HIVT_CHECK_LAUNCH(what);
+    hipLaunchKernelGGL(table_kernel, dim3(a.H, (a.buckets + 63) / 64), dim3(1024), 0, stream, a, partial, w.groups,
+                       a.d_table);
+    HIVT_CHECK_LAUNCH(what);
+  }
+  return HIVT_OK;
+}
+
+template <typename T, int DP>
+int launch_width(const Args& a, char* ws, const Work& w, hipStream_t stream) {
+  using TL = Tile<T, DP>;
+  // 32 keys to a wave where its operands and sums fit the registers (fp32 at 128 wide: they do not)
+  constexpr int KB = sizeof(T) == 4 && DP >= 96 ? 1 : 2, BQ = 32;
+  const char* what = "hivt_relative_attn_bwd";
+  const int rc = rows_per_group(a.M) == 16 ? launch_rows<T, DP, 1>(a, ws, w, stream) : launch_rows<T, DP, 2>(a, ws, w, stream);
+  if (rc != HIVT_OK || a.N == 0) return rc;
+  const int64_t blocks = (int64_t)a.B * a.G * ((a.N + 64 * KB - 1) / (64 * KB));
+  const size_t lds = (size_t)2 * BQ * TL::PITCH * sizeof(T) + BQ * sizeof(float4) + (size_t)bias_width(a) * sizeof(float);
+  HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
+  if (lds > 48 * 1024)
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&dkv_kernel<T, DP, KB, BQ>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
+  hipLaunchKernelGGL((dkv_kernel<T, DP, KB, BQ>), dim3((unsigned)blocks), dim3(256), lds, stream, a);
+  HIVT_CHECK_LAUNCH(what);
+  return HIVT_OK;
+}
+
+template <typename T>
+int launch_type(const Args& a, char* ws, const Work& w, hipStream_t stream) {
+  if (a.d <= 16) return launch_width<T, 16>(a, ws, w, stream);
+  if (a.d <= 32) return launch_width<T, 32>(a, ws, w, stream);
+  if (a.d <= 64) return launch_width<T, 64>(a, ws, w, stream);
+  if (a.d <= 96) return launch_width<T, 96>(a, ws, w, stream);
+  return launch_width<T, 128>(a, ws, w, stream);
+}
+
+}  // namespace
+
+int from_public(const char* what, const hivt_relative_attn* p, const int32_t* starts, float scale, Args& a);
+
+}  // namespace rel
+}  // namespace hivt
+
+using namespace hivt;
+using namespace hivt::rel;
+
+extern "C" size_t hivt_relative_attn_bwd_workspace_bytes(const hivt_relative_attn* p, const int32_t* starts) {
+  Args a;
+  if (from_public("hivt_relative_attn_bwd", p, starts, 1.0f, a) != HIVT_OK) return 0;
+  return work_of(a).total;
+}
+
+extern "C" int hivt_relative_attn_bwd(const hivt_relative_attn* p, const int32_t* starts, float scale, void* workspace,
+                                      size_t workspace_bytes, hivt_stream_t stream) {
+  const char* what = "hivt_relative_attn_bwd";
+  Args a;
+  const int rc = from_public(what, p, starts, scale, a);
+  if (rc != HIVT_OK) return rc;
+  HIVT_REQUIRE(a.B == 0 || a.M == 0 || (a.q && a.table && a.out && a.stats && a.d_out && a.dq), HIVT_ERR_ARG,
+               "%s: null pointer", what);
+  HIVT_REQUIRE(a.B == 0 || a.N == 0 || (a.k && a.v && a.dk && a.dv), HIVT_ERR_ARG, "%s: null pointer", what);
+  HIVT_REQUIRE(a.B > 0 && a.M > 0, HIVT_ERR_ARG, "%s: no query rows: the gradients are zero", what);
+  const Work w = work_of(a);
+  HIVT_REQUIRE(workspace != nullptr && workspace_bytes >= w.total, HIVT_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, w.total);
+  char* const ws = static_cast<char*>(workspace);
+  a.delta = reinterpret_cast<float*>(ws + w.delta);
+  switch (p->dtype) {
+    case HIVT_F32: return launch_type<float>(a, ws, w, (hipStream_t)stream);
+    case HIVT_BF16: return launch_type<__bf16>(a, ws, w, (hipStream_t)stream);
+    default: return launch_type<_Float16>(a, ws, w, (hipStream_t)stream);
+  }
+}

@@ -37,6 +37,7 @@ extern "C" {
 
 #define HIVT_F32 0
 #define HIVT_BF16 1
+#define HIVT_F16 2
 
 typedef void* hivt_stream_t; /* hipStream_t */
 
@@ -539,6 +540,43 @@ int hivt_temporal_attn_bwd(const float* d_out, const float* qkv, const float* ou
 int hivt_temporal_attn_bwd_half(const float* d_out, const float* qkv, const float* out, const float* lse, int32_t S,
                                 int32_t N, int32_t D, int32_t H, float dropout_p, uint64_t seed,
                                 const uint64_t* seed_ptr, void* d_qkv, hivt_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention with a learned bias for each bucket of relative positions (histories of any length)
+ *
+ *   s[i,j] = scale q_i . k_j + table[bucket(j - (i + q_offset))][h],  p = softmax over the allowed keys,  o = p v
+ * for q [batch, q_len, heads, head_dim] and k, v [batch, k_len, kv_heads, head_dim] (heads a multiple of kv_heads:
+ * query head h reads key head h / (heads / kv_heads)), any strides, the head dimension contiguous.  A key is allowed
+ * if key_mask[b][j] == 0 (null: all) and, with causal != 0, j <= i + q_offset.  A row without an allowed key gives
+ * zeros and passes no gradient.  What masked keys and values hold does not matter, NaN and infinities included.
+ * Buckets of a distance n on one side: n itself below `exact`, else exact + the number of border distances <= n
+ * (`starts` of them, ascending, in the host array); with bidirectional != 0 keys behind the query (j > i + q_offset)
+ * take the second half of the `buckets`, otherwise they count as distance 0.  The last border distance is at most 4096.
+ * All members are 64-bit integers: addresses of device memory, sizes, and strides in elements (batch, position, head).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  int64_t dtype; /* HIVT_F32, HIVT_BF16 or HIVT_F16: q, k, v, out and their gradients */
+  int64_t batch, q_len, k_len, heads, kv_heads, head_dim;
+  int64_t causal, bidirectional, q_offset;
+  int64_t buckets, exact, starts;
+  int64_t q, q_stride[3], k, k_stride[3], v, v_stride[3];
+  int64_t table;                 /* float [buckets][heads] */
+  int64_t key_mask, mask_stride; /* uint8 [batch][k_len], rows mask_stride apart; address 0: no mask */
+  int64_t out, out_stride[3];
+  int64_t stats;                 /* float2 [batch * heads][q_len], written by the forward (0: not wanted) */
+  /* backward only; dk, dv and d_table may be 0 together with nothing else */
+  int64_t d_out, d_out_stride[3], dq, dq_stride[3], dk, dk_stride[3], dv, dv_stride[3];
+  int64_t d_table;               /* float [buckets][heads]; 0: not wanted */
+} hivt_relative_attn;
+
+size_t hivt_relative_attn_fwd_workspace_bytes(const hivt_relative_attn* p, const int32_t* starts);
+int hivt_relative_attn_fwd(const hivt_relative_attn* p, const int32_t* starts, float scale, void* workspace,
+                           size_t workspace_bytes, hivt_stream_t stream);
+
+/* Gradients dq, dk, dv and (if wanted) d_table from d_out, the forward's inputs, its out and stats. */
+size_t hivt_relative_attn_bwd_workspace_bytes(const hivt_relative_attn* p, const int32_t* starts);
+int hivt_relative_attn_bwd(const hivt_relative_attn* p, const int32_t* starts, float scale, void* workspace,
+                           size_t workspace_bytes, hivt_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Fused regression / classification loss (min over modes + Laplace NLL + soft-target CE)
