@@ -579,6 +579,32 @@ int hivt_relative_attn_bwd(const hivt_relative_attn* p, const int32_t* starts, f
                            size_t workspace_bytes, hivt_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Norm of every head of queries and keys, and the rotation of its first components by position
+ *
+ *   y = R(position) (weight * x / sqrt(mean x^2 + eps)): rotary_dim / 2 pairs of components, (i, i + rotary_dim / 2) or,
+ *   interleaved != 0, (2 i, 2 i + 1), turned by position * rates[i] (host array of rotary_dim / 2 doubles).
+ * q [batch, length, heads, head_dim] and k [batch, length, kv_heads, head_dim], any strides, the head dimension contiguous
+ * and even, at most 256.  Positions: int32 or int64 (position_bytes 4 or 8) by batch and row, or,
+ * position_bytes 0, the row's index.  Members as in hivt_relative_attn; the weights and their gradients are float.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  int64_t dtype;
+  int64_t batch, length, heads, kv_heads, head_dim, rotary_dim, interleaved;
+  int64_t q, q_stride[3], k, k_stride[3];
+  int64_t q_weight, k_weight; /* float [head_dim] */
+  int64_t positions, position_stride[2], position_bytes;
+  int64_t q_out, q_out_stride[3], k_out, k_out_stride[3]; /* forward */
+  /* backward: from the outputs' gradients and the forward's inputs; the float gradients of the weights are overwritten */
+  int64_t d_q_out, d_q_out_stride[3], d_k_out, d_k_out_stride[3], dq, dq_stride[3], dk, dk_stride[3];
+  int64_t dq_weight, dk_weight;
+} hivt_qk_norm_rotary;
+
+int hivt_qk_norm_rotary_fwd(const hivt_qk_norm_rotary* p, const double* rates, float eps, hivt_stream_t stream);
+size_t hivt_qk_norm_rotary_bwd_workspace_bytes(int64_t head_dim);
+int hivt_qk_norm_rotary_bwd(const hivt_qk_norm_rotary* p, const double* rates, float eps, void* workspace,
+                            size_t workspace_bytes, hivt_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Fused regression / classification loss (min over modes + Laplace NLL + soft-target CE)
  * ------------------------------------------------------------------------------------------ */
 

@@ -40,3 +40,15 @@ def test_relative_attention_argument_block_matches_the_header():
             size = re.search(r"\[(\d+)\]", name)
             members += int(size.group(1)) if size else 1
     assert ctypes.sizeof(ops_relative._Block) == 8 * members
+
+
+def test_rotary_argument_block_matches_the_header():
+    header = open(os.path.join(ROOT, "include", "hivt_mi355.h")).read()
+    from hivt_gan_amd import ops_rotary
+    body = re.search(r"typedef struct \{((?:(?!typedef struct).)*?)\} hivt_qk_norm_rotary;", header, re.S).group(1)
+    members = 0
+    for decl in re.findall(r"int64_t ([^;]*);", re.sub(r"/\*.*?\*/", "", body, flags=re.S)):
+        for name in decl.split(","):
+            size = re.search(r"\[(\d+)\]", name)
+            members += int(size.group(1)) if size else 1
+    assert ctypes.sizeof(ops_rotary._Block) == 8 * members
