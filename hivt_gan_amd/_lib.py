@@ -129,6 +129,8 @@ SIGNATURES = {
     "hivt_qk_norm_rotary_fwd": (c_int, [_P, _P, c_float, _P]),
     "hivt_qk_norm_rotary_bwd_workspace_bytes": (c_size_t, [c_int64]),
     "hivt_qk_norm_rotary_bwd": (c_int, [_P, _P, c_float, _P, c_size_t, _P]),
+    "hivt_orthogonalize_workspace_bytes": (c_size_t, [_P, c_int32]),
+    "hivt_orthogonalize": (c_int, [_P, c_int32, c_int32, c_int32, c_float, _P, c_size_t, _P]),
     "hivt_set_matmul_bf16": (c_int, [c_int]),
     "hivt_spectral_norm_fwd": (c_int, [c_int32, _P, _P, _P, _P, _P, c_int32, c_float, _P, _P, _P, _P, _P]),
     "hivt_spectral_norm_bwd": (c_int, [c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P]),

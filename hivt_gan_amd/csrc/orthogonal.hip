@@ -1,0 +1,529 @@
+// Orthogonalised updates: five steps of a quintic Newton-Schulz iteration on X / |X|, for a list of matrices.
+//
+//   X <- a X + (b G + c G^2) X,  G = X X'   (X with rows <= columns; a taller matrix enters transposed)
+//
+// Every factor in front of X is a polynomial of G, and polynomials of one symmetric matrix commute, so a phase of several
+// steps can be taken on the small side alone:
+//   P = a + b G + c G^2,  Q <- P Q,  G <- P G P   per step, and X <- Q X once at the end of the phase.
+// With X m x n that costs 3 m^2 n per phase and 5 m^3 or fewer per step (symmetric products at half, only the tiles on and
+// below the diagonal are computed) instead of 3 m^2 n + m^3 per step.  A phase forms G from the rounded X of the phase
+// before: what the squares of small singular values lose in G comes back only there.  Hence the phases' lengths: 2 + 3
+// steps for wide matrices (n >= 2 m) and 16-bit results, 1 + 2 + 2 for nearly square fp32 ones, where it costs the same
+// (20 m^3) and a graded spectrum needs it (64 x 64, columns falling to 1e-3: 7e-7 instead of 4e-6).  One phase of five
+// would save another third, but is 5e-3 off on matrices of low rank, even for 16-bit results too much.
+//
+// Bound by the matrix cores.  fp32 ones are eight times slower than 16-bit ones, so a value x is kept as two fp16 numbers
+// (hi = fp16(s x), lo = fp16(s x - hi)) and a product is hi hi + hi lo + lo hi with fp32 sums: 2^-24 of the value per
+// operand, as fp32, at three matrix instructions.  bfloat16 halves would keep 16 bits only.  fp16's range is no concern:
+// the iteration keeps all singular values below 1.21, so the scale s is known beforehand.  (One fp16 product alone is
+// not enough even for 16-bit results: 5e-2 on matrices of low rank, whose small singular values the iteration lifts.)
+//
+// All operands are stored with the reduction index contiguous, which X X' and the symmetric products have anyway; for Q X
+// the transposed X is kept as well (written by the same epilogue).  Planes are padded to multiples of 64 with zeros.
+#include "common.h"
+
+#include <math.h>
+#include <string.h>
+
+namespace hivt {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kMats = 72;        // matrices per launch (descriptors travel in the argument block)
+constexpr int kPad = 64;
+constexpr int kSumChunk = 16384; // elements of a workgroup of the norm
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+
+struct Mat {
+  const void* in;
+  void* out;
+  int64_t ws;        // byte offset of this matrix's workspace
+  int32_t rows, cols;
+  int32_t first;     // first workgroup of this matrix in the launch
+  int32_t pad_;
+};
+struct Group {
+  Mat mats[kMats];
+  int32_t count, dtype;
+  char* base;
+  float eps;
+};
+
+// Workspace of a matrix: scalars, partial sums, planes.  A plane pair is [rows padded][columns padded] fp16 twice.
+struct Layout {
+  int32_t m, n, mp, np;    // small side, large side, padded
+  int64_t big, small;      // bytes of a plane pair: X or its transpose; a square one
+  int64_t sums, x, xt0, sq0, total;
+  __host__ __device__ int64_t xt(int i) const { return xt0 + i * big; }
+  __host__ __device__ int64_t sq(int i) const { return sq0 + i * small; }
+};
+__host__ __device__ inline int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+__host__ __device__ inline Layout layout_of(int32_t rows, int32_t cols) {
+  Layout l;
+  l.m = rows < cols ? rows : cols;
+  l.n = rows < cols ? cols : rows;
+  l.mp = (int32_t)up(l.m, kPad);
+  l.np = (int32_t)up(l.n, kPad);
+  l.big = (int64_t)l.mp * l.np * 4;
+  l.small = (int64_t)l.mp * l.mp * 4;
+  l.sums = 256;
+  const int64_t at = l.sums + up(((int64_t)rows * cols + kSumChunk - 1) / kSumChunk * 8, 256);
+  l.x = at;
+  l.xt0 = at + l.big;
+  l.sq0 = l.xt0 + 2 * l.big;
+  l.total = up(l.sq0 + 5 * l.small, 256);
+  return l;
+}
+
+__device__ __forceinline__ int which(const Group& g, int block) {
+  int i = 0;
+  while (i + 1 < g.count && g.mats[i + 1].first <= block) ++i;
+  return i;
+}
+
+__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
+  if (dtype == HIVT_F32) return static_cast<const float*>(p)[i];
+  if (dtype == HIVT_BF16) return (float)static_cast<const __bf16*>(p)[i];
+  return (float)static_cast<const _Float16*>(p)[i];
+}
+
+// sums of squares, in 64 bits: squares of small or large gradients leave the range of fp32
+__global__ __launch_bounds__(256) void sum_kernel(const Group g) {
+  __shared__ double red[4];
+  const int i = which(g, blockIdx.x);
+  const Mat& a = g.mats[i];
+  const int64_t total = (int64_t)a.rows * a.cols, from = (int64_t)(blockIdx.x - a.first) * kSumChunk;
+  const int64_t to = from + kSumChunk < total ? from + kSumChunk : total;
+  double s = 0.0;
+  for (int64_t j = from + threadIdx.x; j < to; j += 256) {
+    const double v = load_as_float(a.in, j, g.dtype);
+    s += v * v;
+  }
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double* sums = reinterpret_cast<double*>(g.base + a.ws + layout_of(a.rows, a.cols).sums);
+    sums[blockIdx.x - a.first] = red[0] + red[1] + red[2] + red[3];
+  }
+}
+
+// Exponent of the scale of X's planes after `taken` steps: the spectral norm is at most 1.21, and at most x0 a^taken
+// where |X| / (|X| + eps) = x0 is small (a matrix near or below eps keeps its relative precision).
+__device__ __forceinline__ int x_exponent(float x0, int taken) {
+  float bound = x0;
+  for (int i = 0; i < taken; ++i) bound = fminf(bound * kA, 1.0f);
+  if (!(bound > 0.0f)) return 14;
+  const int k = -(int)floorf(log2f(bound)) - 1;
+  return 14 + (k > 0 ? (k < 100 ? k : 100) : 0);
+}
+
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  lo = (_Float16)(v - (float)hi);
+}
+
+// x / (|x| + eps) into the planes of X and of its transpose, a 64 x 64 tile per workgroup
+__global__ __launch_bounds__(256) void convert_kernel(const Group g) {
+  __shared__ float tile[64][65];
+  __shared__ double red[4];
+  const int i = which(g, blockIdx.x);
+  const Mat& a = g.mats[i];
+  const Layout l = layout_of(a.rows, a.cols);
+  char* const ws = g.base + a.ws;
+  const double* sums = reinterpret_cast<const double*>(ws + l.sums);
+  const int parts = (int)(((int64_t)a.rows * a.cols + kSumChunk - 1) / kSumChunk);
+  double s = 0.0;
+  for (int j = threadIdx.x; j < parts; j += 256) s += sums[j];
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
+  const float x0 = (float)(norm / (norm + g.eps));
+  const int block = blockIdx.x - a.first;
+  if (block == 0 && threadIdx.x == 0) *reinterpret_cast<float*>(ws) = x0;
+  const double factor = ldexp(1.0 / (norm + g.eps), x_exponent(x0, 0));
+  const bool flip = a.rows > a.cols;
+  const int tc = l.np / 64, i0 = block / tc * 64, j0 = block % tc * 64;  // of the small x large form
+  // read along the rows of the matrix as it lies
+  for (int e = threadIdx.x; e < 4096; e += 256) {
+    const int r = e >> 6, c = e & 63;
+    const int row = (flip ? j0 : i0) + r, col = (flip ? i0 : j0) + c;
+    const float v = row < a.rows && col < a.cols
+                        ? (float)(load_as_float(a.in, (int64_t)row * a.cols + col, g.dtype) * factor) : 0.0f;
+    tile[flip ? c : r][flip ? r : c] = v;
+  }
+  __syncthreads();
+  _Float16* const x = reinterpret_cast<_Float16*>(ws + l.x);
+  _Float16* const xt = reinterpret_cast<_Float16*>(ws + l.xt(0));
+  const int64_t plane = (int64_t)l.mp * l.np;
+  for (int e = threadIdx.x; e < 4096; e += 256) {
+    const int r = e >> 6, c = e & 63;
+    _Float16 hi, lo;
+    split(tile[r][c], hi, lo);
+    int64_t at = (int64_t)(i0 + r) * l.np + j0 + c;
+    x[at] = hi;
+    x[plane + at] = lo;
+    split(tile[c][r], hi, lo);
+    at = (int64_t)(j0 + r) * l.mp + i0 + c;
+    xt[at] = hi;
+    xt[plane + at] = lo;
+  }
+}
+
+// One product for every matrix of the group: dst = alpha A B' + beta R + diag I, all as planes; A, B with the reduction
+// index contiguous.
+enum Shape : int { SHAPE_GRAM, SHAPE_SQUARE, SHAPE_APPLY };  // X X';  small x small;  Q X (as Q Xt')
+struct Product {
+  int32_t shape;
+  int32_t a, b, dst;     // SQUARE: which of the five square planes; GRAM: dst; APPLY: a
+  int32_t from, to;      // APPLY / GRAM: which transposed planes hold X / get the result
+  int32_t r;             // SQUARE: the planes added with beta, or -1
+  int32_t ea, eb, ed, er;  // exponents of the planes' scales (of square planes)
+  int32_t taken, taken_after;  // steps that X has taken before / after (its scale)
+  int32_t last;          // APPLY: the result is the output
+  float alpha, beta, diag;
+};
+
+template <int BM> struct Cfg {
+  static constexpr int BK = 32;
+  static constexpr int WT = BM / 2;        // a wave's square
+  static constexpr int NT = WT / 32;       // 32 x 32 blocks along it
+  static constexpr int PLANE = BM * BK;    // halves of an operand plane in LDS
+  static constexpr int NPT = BM * BK * 2 / 16 / 256;  // 16-byte pieces of a plane per thread
+};
+
+// rows of 32 halves; the four 16-byte pieces of a row trade places by the row's bits 2-3, so that sixteen consecutive
+// rows read at one column start on sixteen groups of four banks
+__device__ __forceinline__ int lds_at(int row, int piece) { return row * 32 + (((piece ^ (row >> 2)) & 3) << 3); }
+
+template <int BM>
+__global__ __launch_bounds__(256) void product_kernel(const Group g, const Product p) {
+  using C = Cfg<BM>;
+  __shared__ __attribute__((aligned(16))) _Float16 lds[2][4][C::PLANE];  // A hi, A lo, B hi, B lo; double-buffered
+  const int gi = which(g, blockIdx.x);
+  const Mat& mat = g.mats[gi];
+  const Layout l = layout_of(mat.rows, mat.cols);
+  char* const ws = g.base + mat.ws;
+  const int block = blockIdx.x - mat.first;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float x0 = *reinterpret_cast<const float*>(ws);
+
+  const bool apply = p.shape == SHAPE_APPLY, gram = p.shape == SHAPE_GRAM;
+  const int M = l.mp, N = apply ? l.np : l.mp, K = gram ? l.np : l.mp;
+  int ti, tj;
+  if (apply) {
+    const int tiles = (N + BM - 1) / BM;
+    ti = block / tiles;
+    tj = block % tiles;
+  } else {  // tiles on and below the diagonal
+    ti = (int)((sqrtf(8.0f * (float)block + 1.0f) - 1.0f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= block) ++ti;
+    while (ti * (ti + 1) / 2 > block) --ti;
+    tj = block - ti * (ti + 1) / 2;
+  }
+  const int i0 = ti * BM, j0 = tj * BM;
+  const int64_t big = (int64_t)l.mp * l.np, small = (int64_t)l.mp * l.mp;
+  const _Float16* A = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : l.sq(p.a)));
+  const _Float16* B = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : apply ? l.xt(p.from) : l.sq(p.b)));
+  const int64_t planeA = gram ? big : small, planeB = gram || apply ? big : small;
+
+  uint4 regs[4][C::NPT];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < C::NPT; ++i) {
+      const int idx = tid + i * 256, row = idx >> 2, piece = idx & 3;
+      // (a 128-row tile may reach past the planes, which are padded to 64: those rows repeat the last and are not stored)
+      const int64_t ra = (int64_t)min(i0 + row, M - 1) * K + k0 + piece * 8, rb = (int64_t)min(j0 + row, N - 1) * K + k0 + piece * 8;
+      regs[0][i] = *reinterpret_cast<const uint4*>(A + ra);
+      regs[1][i] = *reinterpret_cast<const uint4*>(A + planeA + ra);
+      regs[2][i] = *reinterpret_cast<const uint4*>(B + rb);
+      regs[3][i] = *reinterpret_cast<const uint4*>(B + planeB + rb);
+    }
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < C::NPT; ++i) {
+      const int idx = tid + i * 256;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(&lds[buf][q][lds_at(idx >> 2, idx & 3)]) = regs[q][i];
+    }
+  };
+
+  f32x16 acc[C::NT][C::NT];
+#pragma unroll
+  for (int i = 0; i < C::NT; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  const int wi = (wave >> 1) * C::WT, wj = (wave & 1) * C::WT;
+
+  fetch(0);
+  put(0);
+  __syncthreads();
+  const int steps = K / C::BK;
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1;
+    if (s + 1 < steps) fetch((s + 1) * C::BK);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      f16x8 fa[2][C::NT], fb[2][C::NT];
+      const int piece = ks * 2 + (lane >> 5);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < C::NT; ++i) {
+          fa[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][q][lds_at(wi + i * 32 + (lane & 31), piece)]);
+          fb[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][2 + q][lds_at(wj + i * 32 + (lane & 31), piece)]);
+        }
+#pragma unroll
+      for (int i = 0; i < C::NT; ++i)
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
+        }
+    }
+    if (s + 1 < steps) put(buf ^ 1);  // (that buffer's readers passed the barrier of the step before)
+    __syncthreads();
+  }
+
+  // results: column = lane & 31, rows 8 (e / 4) + 4 (lane >> 5) + e % 4 of a 32 x 32 block
+  const int ex = x_exponent(x0, p.taken), ex_after = x_exponent(x0, p.taken_after);
+  const int down = gram ? 2 * ex : apply ? p.ea + ex : p.ea + p.eb;
+  const float unscale = ldexpf(p.alpha, -down);
+  const int ed = apply ? ex_after : p.ed;
+  const _Float16* R = p.r >= 0 ? reinterpret_cast<const _Float16*>(ws + l.sq(p.r)) : nullptr;
+  const float rscale = ldexpf(p.beta, -p.er);
+#pragma unroll
+  for (int bi = 0; bi < C::NT; ++bi)
+#pragma unroll
+    for (int bj = 0; bj < C::NT; ++bj)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int row = i0 + wi + bi * 32 + e4 * 8 + (lane >> 5) * 4, col = j0 + wj + bj * 32 + (lane & 31);
+        if (row >= M || col >= N) continue;
+        float v[4];
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[bi][bj][e4 * 4 + e] * unscale;
+          if (!apply) {
+            if (R != nullptr) {
+              const int64_t at = (int64_t)(row + e) * l.mp + col;
+              v[e] += rscale * ((float)R[at] + (float)R[small + at]);
+            }
+            if (row + e == col) v[e] += p.diag;
+          }
+          const bool in = row + e < l.m && col < (apply ? l.n : l.m);
+          if (!in) v[e] = 0.0f;
+        }
+        if (apply && p.last) {
+          const bool flip = mat.rows > mat.cols;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (row + e >= l.m || col >= l.n) continue;
+            const int64_t at = flip ? (int64_t)col * l.m + row + e : (int64_t)(row + e) * l.n + col;
+            if (g.dtype == HIVT_F32) static_cast<float*>(mat.out)[at] = v[e];
+            else if (g.dtype == HIVT_BF16) static_cast<__bf16*>(mat.out)[at] = (__bf16)v[e];
+            else static_cast<_Float16*>(mat.out)[at] = (_Float16)v[e];
+          }
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          _Float16 h, o;
+          split(ldexpf(v[e], ed), h, o);
+          hi[e] = h;
+          lo[e] = o;
+        }
+        // as it stands, and transposed (the square results are symmetric: the tile above the diagonal)
+        _Float16* dst = reinterpret_cast<_Float16*>(ws + (apply ? l.x : l.sq(p.dst)));
+        _Float16* dt = reinterpret_cast<_Float16*>(ws + (apply ? l.xt(p.to) : l.sq(p.dst)));
+        const int64_t plane = apply ? big : small;
+        const int ld = apply ? l.np : l.mp;
+        if (apply || ti >= tj) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            dst[(int64_t)(row + e) * ld + col] = hi[e];
+            dst[plane + (int64_t)(row + e) * ld + col] = lo[e];
+          }
+        }
+        if (apply || ti != tj) {
+          *reinterpret_cast<f16x4*>(dt + (int64_t)col * l.mp + row) = hi;
+          *reinterpret_cast<f16x4*>(dt + plane + (int64_t)col * l.mp + row) = lo;
+        }
+      }
+}
+
+int64_t tiles_of(const Mat& a, int shape, int bm) {
+  const Layout l = layout_of(a.rows, a.cols);
+  const int64_t tm = (l.mp + bm - 1) / bm, tn = (l.np + bm - 1) / bm;
+  return shape == SHAPE_APPLY ? tm * tn : tm * (tm + 1) / 2;
+}
+
+int launch_product(Group& g, const Product& p, hipStream_t stream) {
+  const char* what = "hivt_orthogonalize";
+  int64_t wide = 0;
+  for (int i = 0; i < g.count; ++i) wide += tiles_of(g.mats[i], p.shape, 128);
+  const int bm = wide >= 256 ? 128 : 64;  // the larger tile once it fills the compute units
+  int64_t blocks = 0;
+  for (int i = 0; i < g.count; ++i) {
+    g.mats[i].first = (int32_t)blocks;
+    blocks += tiles_of(g.mats[i], p.shape, bm);
+    HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
+  }
+  if (bm == 128) hipLaunchKernelGGL(product_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, g, p);
+  else hipLaunchKernelGGL(product_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, g, p);
+  HIVT_CHECK_LAUNCH(what);
+  return HIVT_OK;
+}
+
+// exponent of the scale of a product of k factors P (each at most 3.45)
+int q_exponent(int k) { return 16 - 2 * k; }
+
+int run_group(Group& g, const int* phases, int nphases, hipStream_t stream) {
+  const char* what = "hivt_orthogonalize";
+  int64_t blocks = 0;
+  for (int i = 0; i < g.count; ++i) {
+    g.mats[i].first = (int32_t)blocks;
+    blocks += ((int64_t)g.mats[i].rows * g.mats[i].cols + kSumChunk - 1) / kSumChunk;
+  }
+  HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
+  hipLaunchKernelGGL(sum_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, g);
+  HIVT_CHECK_LAUNCH(what);
+  blocks = 0;
+  for (int i = 0; i < g.count; ++i) {
+    g.mats[i].first = (int32_t)blocks;
+    const Layout l = layout_of(g.mats[i].rows, g.mats[i].cols);
+    blocks += (int64_t)(l.mp / 64) * (l.np / 64);
+  }
+  HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
+  hipLaunchKernelGGL(convert_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, g);
+  HIVT_CHECK_LAUNCH(what);
+
+  int taken = 0, at = 0;
+  for (int f = 0; f < nphases; ++f) {
+    // square planes: 0 G, 1 P G, 2 P, and 3 / 4 in turn Q
+    Product p;
+    memset(&p, 0, sizeof(p));
+    p.r = -1;
+    p.alpha = 1.0f;
+    p.shape = SHAPE_GRAM;
+    p.taken = p.taken_after = taken;
+    p.dst = 0;
+    p.ed = 14;
+    int rc = launch_product(g, p, stream);
+    if (rc != HIVT_OK) return rc;
+    p.shape = SHAPE_SQUARE;
+    int q = 3;
+    for (int s = 0; s < phases[f]; ++s) {
+      auto square = [&](int a, int ea, int b, int eb, int dst, int ed, float alpha, int r, float beta, float diag) {
+        p.a = a; p.ea = ea; p.b = b; p.eb = eb; p.dst = dst; p.ed = ed;
+        p.alpha = alpha; p.r = r; p.er = 14; p.beta = beta; p.diag = diag;
+        return launch_product(g, p, stream);
+      };
+      const int poly = s == 0 ? q : 2;
+      if ((rc = square(0, 14, 0, 14, poly, 14, kC, 0, kB, kA)) != HIVT_OK) return rc;
+      if (s > 0) {
+        if ((rc = square(poly, 14, q, q_exponent(s), 7 - q, q_exponent(s + 1), 1.0f, -1, 0.0f, 0.0f)) != HIVT_OK) return rc;
+        q = 7 - q;
+      }
+      if (s + 1 < phases[f]) {
+        if ((rc = square(poly, 14, 0, 14, 1, 14, 1.0f, -1, 0.0f, 0.0f)) != HIVT_OK) return rc;
+        if ((rc = square(1, 14, poly, 14, 0, 14, 1.0f, -1, 0.0f, 0.0f)) != HIVT_OK) return rc;
+      }
+    }
+    memset(&p, 0, sizeof(p));
+    p.r = -1;
+    p.alpha = 1.0f;
+    p.shape = SHAPE_APPLY;
+    p.a = q;
+    p.ea = q_exponent(phases[f]);
+    p.from = at;
+    p.to = at ^ 1;
+    p.taken = taken;
+    p.taken_after = taken + phases[f];
+    p.last = f + 1 == nphases;
+    if ((rc = launch_product(g, p, stream)) != HIVT_OK) return rc;
+    taken += phases[f];
+    at ^= 1;
+  }
+  return HIVT_OK;
+}
+
+int check(const char* what, const hivt_matrix* list, int32_t count, int32_t dtype, int32_t steps) {
+  HIVT_REQUIRE(count >= 0 && (count == 0 || list != nullptr), HIVT_ERR_ARG, "%s: bad list", what);
+  HIVT_REQUIRE(dtype == HIVT_F32 || dtype == HIVT_BF16 || dtype == HIVT_F16, HIVT_ERR_UNSUPPORTED, "%s: element type %d",
+               what, (int)dtype);
+  HIVT_REQUIRE(steps >= 1 && steps <= 16, HIVT_ERR_ARG, "%s: %d steps (1 to 16)", what, (int)steps);
+  for (int32_t i = 0; i < count; ++i)
+    HIVT_REQUIRE(list[i].rows >= 0 && list[i].cols >= 0 && list[i].rows <= 65536 && list[i].cols <= 65536, HIVT_ERR_ARG,
+                 "%s: matrix %d is %lld x %lld (at most 65536)", what, (int)i, (long long)list[i].rows, (long long)list[i].cols);
+  return HIVT_OK;
+}
+
+}  // namespace
+}  // namespace hivt
+
+using namespace hivt;
+
+extern "C" size_t hivt_orthogonalize_workspace_bytes(const hivt_matrix* list, int32_t count) {
+  if (check("hivt_orthogonalize", list, count, HIVT_F32, 1) != HIVT_OK) return 0;
+  int64_t total = 0;
+  for (int32_t i = 0; i < count; ++i)
+    if (list[i].rows > 0 && list[i].cols > 0) total += layout_of((int32_t)list[i].rows, (int32_t)list[i].cols).total;
+  return (size_t)total;
+}
+
+extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_t dtype, int32_t steps, float eps,
+                                  void* workspace, size_t workspace_bytes, hivt_stream_t stream) {
+  const char* what = "hivt_orthogonalize";
+  int rc = check(what, list, count, dtype, steps);
+  if (rc != HIVT_OK) return rc;
+  HIVT_REQUIRE(eps > 0.0f, HIVT_ERR_ARG, "%s: eps must be positive", what);
+  const size_t need = hivt_orthogonalize_workspace_bytes(list, count);
+  HIVT_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), HIVT_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  for (int32_t i = 0; i < count; ++i)
+    HIVT_REQUIRE(list[i].rows * list[i].cols == 0 || (list[i].in && list[i].out), HIVT_ERR_ARG, "%s: null pointer", what);
+  // two kinds of matrices, with phases of up to two or three steps
+  int64_t at = 0;
+  for (int kind = 0; kind < 2; ++kind) {
+    int phases[16], n = 0, left = steps;
+    const int most = kind == 0 ? 2 : 3;
+    if (left % most != 0) { phases[n++] = left % most; left -= left % most; }
+    for (; left > 0; left -= most) phases[n++] = most;
+    Group g;
+    memset(&g, 0, sizeof(g));
+    g.dtype = dtype;
+    g.base = static_cast<char*>(workspace);
+    g.eps = eps;
+    for (int32_t i = 0; i <= count; ++i) {
+      if (i < count) {
+        const int64_t r = list[i].rows, c = list[i].cols;
+        if (r * c == 0) continue;
+        const bool is_wide = r >= 2 * c || c >= 2 * r;
+        if ((dtype == HIVT_F32 ? is_wide : true) != (kind == 1)) continue;
+        Mat& m = g.mats[g.count++];
+        m.in = reinterpret_cast<const void*>(list[i].in);
+        m.out = reinterpret_cast<void*>(list[i].out);
+        m.rows = (int32_t)r;
+        m.cols = (int32_t)c;
+        m.ws = at;
+        at += layout_of(m.rows, m.cols).total;
+      }
+      if (g.count > 0 && (i == count || g.count == kMats)) {
+        rc = run_group(g, phases, n, (hipStream_t)stream);
+        if (rc != HIVT_OK) return rc;
+        g.count = 0;
+      }
+    }
+  }
+  return HIVT_OK;
+}

@@ -28,6 +28,7 @@ from .ops_edges import (  # noqa: F401  (every name stays reachable as ops.<name
 from .ops_losses import (  # noqa: F401  (every name stays reachable as ops.<name>)
     _SupervisedLoss, supervised_loss, supervised_loss_packed, _HingeR1Loss, hinge_r1_loss,
     _WeightedMean, weighted_mean, _HingeR1Multi, hinge_r1_multi, _GeneratorTotal, generator_total)
+from .ops_orthogonal import orthogonalize  # noqa: F401
 from .ops_relative import relative_attention, relative_buckets, relative_self_attention  # noqa: F401
 from .ops_rotary import qk_norm_rotary  # noqa: F401
 from .ops_spectral import (  # noqa: F401  (every name stays reachable as ops.<name>)

@@ -1,0 +1,66 @@
+"""Orthogonalised updates of matrices (``hivt_orthogonalize``), what ``optim.Muon`` steps along."""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Sequence
+
+import torch
+
+from . import _lib
+from ._opsbase import _need_gpu, _on_device, _p, _stream, _unsupported, _workspace
+from .ops_relative import _DTYPES
+
+_MAX_SIDE = 65536
+
+
+def matrix_list(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor]):
+    """The ``hivt_matrix`` array of contiguous matrices."""
+    flat = []
+    for x, y in zip(ins, outs):
+        flat += (x.data_ptr(), y.data_ptr(), x.shape[0], x.shape[1])
+    return (ctypes.c_int64 * max(1, len(flat)))(*flat)
+
+
+@torch.no_grad()
+def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float = 1e-7,
+                  out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
+    """Each matrix [rows, cols] of the list, its singular values brought near 1: ``x / (|x| + eps)`` (Frobenius norm), then
+    ``steps`` times ``x <- a x + (b g + c g^2) x`` with g = x x^T (of the shorter side) and a, b, c = 3.4445, -4.7750,
+    2.0315.  One type for the list, float32, bfloat16 or float16; any shapes up to 65536 a side.  The arithmetic is that of
+    fp32 whatever the type, rounded once at the end; results are the same whatever else is in the list.  ``out``:
+    contiguous tensors to write to (the matrices themselves are allowed).  Not differentiable."""
+    matrices = list(matrices)
+    if not matrices:
+        return []
+    dtype, device = matrices[0].dtype, matrices[0].device
+    for x in matrices:
+        if x.dtype not in _DTYPES or x.dtype != dtype:
+            raise TypeError(f"the matrices must share one of float32, bfloat16, float16, got {x.dtype}")
+        if x.dim() != 2:
+            raise ValueError(f"expected matrices, got shape {tuple(x.shape)}")
+        if max(x.shape) > _MAX_SIDE:
+            raise _unsupported(f"orthogonalising a matrix of {tuple(x.shape)} (at most {_MAX_SIDE} a side)")
+        if x.device != device:
+            raise ValueError(f"matrices on {device} and {x.device}")
+    if not 1 <= int(steps) <= 16:
+        raise ValueError(f"steps must be 1 to 16, got {steps}")
+    if not eps > 0.0:
+        raise ValueError(f"eps must be positive, got {eps}")
+    _need_gpu(*matrices)
+    if out is None:
+        out = [torch.empty(x.shape, dtype=dtype, device=device) for x in matrices]
+    else:
+        out = list(out)
+        if len(out) != len(matrices):
+            raise ValueError(f"{len(matrices)} matrices, {len(out)} outputs")
+        for x, y in zip(matrices, out):
+            if y.shape != x.shape or y.dtype != dtype or y.device != device or not y.is_contiguous():
+                raise ValueError(f"an output must be contiguous {dtype} {tuple(x.shape)} on {device}")
+    with _on_device(matrices[0]):
+        ins = [x.contiguous() for x in matrices]
+        array = matrix_list(ins, out)
+        need = _lib.value("hivt_orthogonalize_workspace_bytes", array, len(ins))
+        ws = _workspace(need, device)
+        _lib.call("hivt_orthogonalize", array, len(ins), _DTYPES[dtype], int(steps), float(eps), _p(ws), ws.numel(),
+                  _stream(ins[0]))
+    return out

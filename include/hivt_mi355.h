@@ -605,6 +605,23 @@ int hivt_qk_norm_rotary_bwd(const hivt_qk_norm_rotary* p, const double* rates, f
                             size_t workspace_bytes, hivt_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Orthogonalised updates (Newton-Schulz), for a list of matrices
+ *
+ *   X = in / (|in| + eps) (Frobenius norm), then `steps` times X <- a X + (b G + c G^2) X, G = X X' (X' X for a matrix
+ *   with more rows than columns), with a, b, c = 3.4445, -4.7750, 2.0315: the singular values go near 1.  out = X.
+ * in and out are contiguous row-major matrices of one type; in == out is allowed.  The host array is read before the
+ * call returns.  Results are accurate to fp32 (see the kernels) and do not depend on what else is in the list.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  int64_t in, out;    /* device addresses */
+  int64_t rows, cols; /* at most 65536; an empty matrix is passed over */
+} hivt_matrix;
+
+size_t hivt_orthogonalize_workspace_bytes(const hivt_matrix* list, int32_t count);
+int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_t dtype, int32_t steps, float eps, void* workspace,
+                       size_t workspace_bytes, hivt_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Fused regression / classification loss (min over modes + Laplace NLL + soft-target CE)
  * ------------------------------------------------------------------------------------------ */
 
