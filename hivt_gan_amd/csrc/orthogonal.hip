@@ -8,9 +8,10 @@
 // With X m x n that costs 3 m^2 n per phase and 5 m^3 or fewer per step (symmetric products at half, only the tiles on and
 // below the diagonal are computed) instead of 3 m^2 n + m^3 per step.  A phase forms G from the rounded X of the phase
 // before: what the squares of small singular values lose in G comes back only there.  Hence the phases' lengths: 2 + 3
-// steps for wide matrices (n >= 2 m) and 16-bit results, 1 + 2 + 2 for nearly square fp32 ones, where it costs the same
-// (20 m^3) and a graded spectrum needs it (64 x 64, columns falling to 1e-3: 7e-7 instead of 4e-6).  One phase of five
-// would save another third, but is 5e-3 off on matrices of low rank, even for 16-bit results too much.
+// steps for n >= 1.5 m (23 instead of 27.5 m^3 at 1.5, 38 instead of 65 at 4); single steps for nearly square matrices,
+// where that costs the same (20 m^3) and is the most accurate (a 64 x 64 one with columns falling to 1e-3: 3e-7 off
+// instead of 4e-6).  One phase of five would save another third of a wide one, but is 5e-3 off on matrices of low rank,
+// even for 16-bit results too much.
 //
 // Bound by the matrix cores.  fp32 ones are eight times slower than 16-bit ones, so a value x is kept as two fp16 numbers
 // (hi = fp16(s x), lo = fp16(s x - hi)) and a product is hi hi + hi lo + lo hi with fp32 sums: 2^-24 of the value per
@@ -18,8 +19,11 @@
 // the iteration keeps all singular values below 1.21, so the scale s is known beforehand.  (One fp16 product alone is
 // not enough even for 16-bit results: 5e-2 on matrices of low rank, whose small singular values the iteration lifts.)
 //
-// All operands are stored with the reduction index contiguous, which X X' and the symmetric products have anyway; for Q X
-// the transposed X is kept as well (written by the same epilogue).  Planes are padded to multiples of 64 with zeros.
+// Every product takes both operands with the reduction index innermost, which X X' and the symmetric products have
+// anyway; for Q X the transposed X is kept as well (written by the same epilogue).  Operands are stored as the products
+// read them: blocks of 64 rows by 32 of the reduction index, hi then lo, 8 KB in a piece, in the order of the LDS image.
+// (Row-major planes cost a factor of six at 4096 columns: rows 8 KB apart meet on one memory channel.)  Sides are padded
+// to multiples of 64 with zeros.
 #include "common.h"
 
 #include <math.h>
@@ -32,9 +36,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kMats = 72;        // matrices per launch (descriptors travel in the argument block)
+constexpr int kMats = 64;        // matrices per launch (descriptors travel in the argument block)
 constexpr int kPad = 64;
-constexpr int kSumChunk = 16384; // elements of a workgroup of the norm
+constexpr int kSumChunk = 8192;  // elements of a workgroup of the norm
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 
 struct Mat {
@@ -42,11 +46,10 @@ struct Mat {
   void* out;
   int64_t ws;        // byte offset of this matrix's workspace
   int32_t rows, cols;
-  int32_t first;     // first workgroup of this matrix in the launch
-  int32_t pad_;
 };
 struct Group {
   Mat mats[kMats];
+  int32_t first[kMats];  // first workgroup of a matrix in the launch
   int32_t count, dtype;
   char* base;
   float eps;
@@ -78,10 +81,10 @@ __host__ __device__ inline Layout layout_of(int32_t rows, int32_t cols) {
   return l;
 }
 
+// the matrix that a workgroup works for: every lane looks at one
 __device__ __forceinline__ int which(const Group& g, int block) {
-  int i = 0;
-  while (i + 1 < g.count && g.mats[i + 1].first <= block) ++i;
-  return i;
+  const int lane = threadIdx.x & 63;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < g.count && g.first[lane] <= block)) - 1);
 }
 
 __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
@@ -95,19 +98,23 @@ __global__ __launch_bounds__(256) void sum_kernel(const Group g) {
   __shared__ double red[4];
   const int i = which(g, blockIdx.x);
   const Mat& a = g.mats[i];
-  const int64_t total = (int64_t)a.rows * a.cols, from = (int64_t)(blockIdx.x - a.first) * kSumChunk;
-  const int64_t to = from + kSumChunk < total ? from + kSumChunk : total;
-  double s = 0.0;
-  for (int64_t j = from + threadIdx.x; j < to; j += 256) {
-    const double v = load_as_float(a.in, j, g.dtype);
-    s += v * v;
+  const int64_t total = (int64_t)a.rows * a.cols, from = (int64_t)(blockIdx.x - g.first[i]) * kSumChunk;
+  const int left = (int)(total - from < kSumChunk ? total - from : kSumChunk);
+  float v[kSumChunk / 256];  // all on their way at once
+#pragma unroll
+  for (int j = 0; j < kSumChunk / 256; ++j) {
+    const int at = threadIdx.x + j * 256;
+    v[j] = at < left ? load_as_float(a.in, from + at, g.dtype) : 0.0f;
   }
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < kSumChunk / 256; ++j) s += (double)v[j] * v[j];
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     double* sums = reinterpret_cast<double*>(g.base + a.ws + layout_of(a.rows, a.cols).sums);
-    sums[blockIdx.x - a.first] = red[0] + red[1] + red[2] + red[3];
+    sums[blockIdx.x - g.first[i]] = red[0] + red[1] + red[2] + red[3];
   }
 }
 
@@ -124,6 +131,15 @@ __device__ __forceinline__ int x_exponent(float x0, int taken) {
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
+}
+
+// Rows of 32 halves; the four 16-byte pieces of a row trade places by the row's bits 2-3, so that sixteen consecutive
+// rows read at one column start on sixteen groups of four banks.
+constexpr int kBlock = 64 * 32;
+__device__ __forceinline__ int lds_at(int row, int piece) { return row * 32 + (((piece ^ (row >> 2)) & 3) << 3); }
+// element (row, k) of an operand with K (a multiple of 64) columns; the lo half is kBlock further
+__device__ __forceinline__ int64_t at_of(int row, int k, int K) {
+  return ((int64_t)(row >> 6) * (K >> 5) + (k >> 5)) * (2 * kBlock) + lds_at(row & 63, k >> 3 & 3) + (k & 7);
 }
 
 // x / (|x| + eps) into the planes of X and of its transpose, a 64 x 64 tile per workgroup
@@ -143,7 +159,7 @@ __global__ __launch_bounds__(256) void convert_kernel(const Group g) {
   __syncthreads();
   const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
   const float x0 = (float)(norm / (norm + g.eps));
-  const int block = blockIdx.x - a.first;
+  const int block = blockIdx.x - g.first[i];
   if (block == 0 && threadIdx.x == 0) *reinterpret_cast<float*>(ws) = x0;
   const double factor = ldexp(1.0 / (norm + g.eps), x_exponent(x0, 0));
   const bool flip = a.rows > a.cols;
@@ -159,18 +175,25 @@ __global__ __launch_bounds__(256) void convert_kernel(const Group g) {
   __syncthreads();
   _Float16* const x = reinterpret_cast<_Float16*>(ws + l.x);
   _Float16* const xt = reinterpret_cast<_Float16*>(ws + l.xt(0));
-  const int64_t plane = (int64_t)l.mp * l.np;
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    _Float16 hi, lo;
-    split(tile[r][c], hi, lo);
-    int64_t at = (int64_t)(i0 + r) * l.np + j0 + c;
-    x[at] = hi;
-    x[plane + at] = lo;
-    split(tile[c][r], hi, lo);
-    at = (int64_t)(j0 + r) * l.mp + i0 + c;
-    xt[at] = hi;
-    xt[plane + at] = lo;
+  for (int e = threadIdx.x; e < 1024; e += 256) {  // four elements at a time
+    const int r = e >> 4, c = (e & 15) * 4;
+    f16x4 hi, lo, hit, lot;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      _Float16 u, v;
+      split(tile[r][c + j], u, v);
+      hi[j] = u;
+      lo[j] = v;
+      split(tile[c + j][r], u, v);
+      hit[j] = u;
+      lot[j] = v;
+    }
+    int64_t at = at_of(i0 + r, j0 + c, l.np);
+    *reinterpret_cast<f16x4*>(x + at) = hi;
+    *reinterpret_cast<f16x4*>(x + at + kBlock) = lo;
+    at = at_of(j0 + r, i0 + c, l.mp);
+    *reinterpret_cast<f16x4*>(xt + at) = hit;
+    *reinterpret_cast<f16x4*>(xt + at + kBlock) = lot;
   }
 }
 
@@ -192,23 +215,19 @@ template <int BM> struct Cfg {
   static constexpr int BK = 32;
   static constexpr int WT = BM / 2;        // a wave's square
   static constexpr int NT = WT / 32;       // 32 x 32 blocks along it
-  static constexpr int PLANE = BM * BK;    // halves of an operand plane in LDS
-  static constexpr int NPT = BM * BK * 2 / 16 / 256;  // 16-byte pieces of a plane per thread
+  static constexpr int TILE = BM / 64 * 2 * kBlock;   // halves of an operand's step in LDS
+  static constexpr int NPT = TILE * 2 / 16 / 256;     // 16-byte pieces of it per thread
 };
-
-// rows of 32 halves; the four 16-byte pieces of a row trade places by the row's bits 2-3, so that sixteen consecutive
-// rows read at one column start on sixteen groups of four banks
-__device__ __forceinline__ int lds_at(int row, int piece) { return row * 32 + (((piece ^ (row >> 2)) & 3) << 3); }
 
 template <int BM>
 __global__ __launch_bounds__(256) void product_kernel(const Group g, const Product p) {
   using C = Cfg<BM>;
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][4][C::PLANE];  // A hi, A lo, B hi, B lo; double-buffered
+  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2][C::TILE];  // A, B; double-buffered
   const int gi = which(g, blockIdx.x);
   const Mat& mat = g.mats[gi];
   const Layout l = layout_of(mat.rows, mat.cols);
   char* const ws = g.base + mat.ws;
-  const int block = blockIdx.x - mat.first;
+  const int block = blockIdx.x - g.first[gi];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float x0 = *reinterpret_cast<const float*>(ws);
 
@@ -226,31 +245,26 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
     tj = block - ti * (ti + 1) / 2;
   }
   const int i0 = ti * BM, j0 = tj * BM;
-  const int64_t big = (int64_t)l.mp * l.np, small = (int64_t)l.mp * l.mp;
   const _Float16* A = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : l.sq(p.a)));
   const _Float16* B = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : apply ? l.xt(p.from) : l.sq(p.b)));
-  const int64_t planeA = gram ? big : small, planeB = gram || apply ? big : small;
-
-  uint4 regs[4][C::NPT];
-  auto fetch = [&](int k0) {
+  // (a 128-row tile may reach past an operand, which is padded to 64 rows: it reads the last block again and does not
+  // store those results)
+  uint4 regs[2][C::NPT];
+  auto fetch = [&](int step) {
 #pragma unroll
     for (int i = 0; i < C::NPT; ++i) {
-      const int idx = tid + i * 256, row = idx >> 2, piece = idx & 3;
-      // (a 128-row tile may reach past the planes, which are padded to 64: those rows repeat the last and are not stored)
-      const int64_t ra = (int64_t)min(i0 + row, M - 1) * K + k0 + piece * 8, rb = (int64_t)min(j0 + row, N - 1) * K + k0 + piece * 8;
-      regs[0][i] = *reinterpret_cast<const uint4*>(A + ra);
-      regs[1][i] = *reinterpret_cast<const uint4*>(A + planeA + ra);
-      regs[2][i] = *reinterpret_cast<const uint4*>(B + rb);
-      regs[3][i] = *reinterpret_cast<const uint4*>(B + planeB + rb);
+      const int idx = tid + i * 256, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;  // block of 64 rows; halves
+      const int64_t ra = (int64_t)min((i0 >> 6) + sub, (M >> 6) - 1) * (K >> 5) + step;
+      const int64_t rb = (int64_t)min((j0 >> 6) + sub, (N >> 6) - 1) * (K >> 5) + step;
+      regs[0][i] = *reinterpret_cast<const uint4*>(A + ra * (2 * kBlock) + in);
+      regs[1][i] = *reinterpret_cast<const uint4*>(B + rb * (2 * kBlock) + in);
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < C::NPT; ++i) {
-      const int idx = tid + i * 256;
+    for (int i = 0; i < C::NPT; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(&lds[buf][q][lds_at(idx >> 2, idx & 3)]) = regs[q][i];
-    }
+      for (int q = 0; q < 2; ++q) *reinterpret_cast<uint4*>(&lds[buf][q][(tid + i * 256) * 8]) = regs[q][i];
   };
 
   f32x16 acc[C::NT][C::NT];
@@ -268,7 +282,7 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
   const int steps = K / C::BK;
   for (int s = 0; s < steps; ++s) {
     const int buf = s & 1;
-    if (s + 1 < steps) fetch((s + 1) * C::BK);
+    if (s + 1 < steps) fetch(s + 1);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       f16x8 fa[2][C::NT], fb[2][C::NT];
@@ -277,8 +291,9 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
       for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int i = 0; i < C::NT; ++i) {
-          fa[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][q][lds_at(wi + i * 32 + (lane & 31), piece)]);
-          fb[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][2 + q][lds_at(wj + i * 32 + (lane & 31), piece)]);
+          const int ra = wi + i * 32 + (lane & 31), rb = wj + i * 32 + (lane & 31);
+          fa[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][0][((ra >> 6) * 2 + q) * kBlock + lds_at(ra & 63, piece)]);
+          fb[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][1][((rb >> 6) * 2 + q) * kBlock + lds_at(rb & 63, piece)]);
         }
 #pragma unroll
       for (int i = 0; i < C::NT; ++i)
@@ -315,8 +330,8 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
           v[e] = acc[bi][bj][e4 * 4 + e] * unscale;
           if (!apply) {
             if (R != nullptr) {
-              const int64_t at = (int64_t)(row + e) * l.mp + col;
-              v[e] += rscale * ((float)R[at] + (float)R[small + at]);
+              const int64_t at = at_of(row + e, col, l.mp);
+              v[e] += rscale * ((float)R[at] + (float)R[at + kBlock]);
             }
             if (row + e == col) v[e] += p.diag;
           }
@@ -345,18 +360,17 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
         // as it stands, and transposed (the square results are symmetric: the tile above the diagonal)
         _Float16* dst = reinterpret_cast<_Float16*>(ws + (apply ? l.x : l.sq(p.dst)));
         _Float16* dt = reinterpret_cast<_Float16*>(ws + (apply ? l.xt(p.to) : l.sq(p.dst)));
-        const int64_t plane = apply ? big : small;
         const int ld = apply ? l.np : l.mp;
-        if (apply || ti >= tj) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            dst[(int64_t)(row + e) * ld + col] = hi[e];
-            dst[plane + (int64_t)(row + e) * ld + col] = lo[e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int64_t at = at_of(row + e, col, ld);
+          dst[at] = hi[e];
+          dst[at + kBlock] = lo[e];
         }
         if (apply || ti != tj) {
-          *reinterpret_cast<f16x4*>(dt + (int64_t)col * l.mp + row) = hi;
-          *reinterpret_cast<f16x4*>(dt + plane + (int64_t)col * l.mp + row) = lo;
+          const int64_t at = at_of(col, row, l.mp);
+          *reinterpret_cast<f16x4*>(dt + at) = hi;
+          *reinterpret_cast<f16x4*>(dt + at + kBlock) = lo;
         }
       }
 }
@@ -374,7 +388,7 @@ int launch_product(Group& g, const Product& p, hipStream_t stream) {
   const int bm = wide >= 256 ? 128 : 64;  // the larger tile once it fills the compute units
   int64_t blocks = 0;
   for (int i = 0; i < g.count; ++i) {
-    g.mats[i].first = (int32_t)blocks;
+    g.first[i] = (int32_t)blocks;
     blocks += tiles_of(g.mats[i], p.shape, bm);
     HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
   }
@@ -391,7 +405,7 @@ int run_group(Group& g, const int* phases, int nphases, hipStream_t stream) {
   const char* what = "hivt_orthogonalize";
   int64_t blocks = 0;
   for (int i = 0; i < g.count; ++i) {
-    g.mats[i].first = (int32_t)blocks;
+    g.first[i] = (int32_t)blocks;
     blocks += ((int64_t)g.mats[i].rows * g.mats[i].cols + kSumChunk - 1) / kSumChunk;
   }
   HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
@@ -399,7 +413,7 @@ int run_group(Group& g, const int* phases, int nphases, hipStream_t stream) {
   HIVT_CHECK_LAUNCH(what);
   blocks = 0;
   for (int i = 0; i < g.count; ++i) {
-    g.mats[i].first = (int32_t)blocks;
+    g.first[i] = (int32_t)blocks;
     const Layout l = layout_of(g.mats[i].rows, g.mats[i].cols);
     blocks += (int64_t)(l.mp / 64) * (l.np / 64);
   }
@@ -492,11 +506,11 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   for (int32_t i = 0; i < count; ++i)
     HIVT_REQUIRE(list[i].rows * list[i].cols == 0 || (list[i].in && list[i].out), HIVT_ERR_ARG, "%s: null pointer", what);
-  // two kinds of matrices, with phases of up to two or three steps
+  // two kinds of matrices: nearly square ones, and wide ones with phases of up to three steps
   int64_t at = 0;
   for (int kind = 0; kind < 2; ++kind) {
     int phases[16], n = 0, left = steps;
-    const int most = kind == 0 ? 2 : 3;
+    const int most = kind == 0 ? 1 : 3;
     if (left % most != 0) { phases[n++] = left % most; left -= left % most; }
     for (; left > 0; left -= most) phases[n++] = most;
     Group g;
@@ -508,8 +522,7 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
       if (i < count) {
         const int64_t r = list[i].rows, c = list[i].cols;
         if (r * c == 0) continue;
-        const bool is_wide = r >= 2 * c || c >= 2 * r;
-        if ((dtype == HIVT_F32 ? is_wide : true) != (kind == 1)) continue;
+        if ((2 * r >= 3 * c || 2 * c >= 3 * r) != (kind == 1)) continue;
         Mat& m = g.mats[g.count++];
         m.in = reinterpret_cast<const void*>(list[i].in);
         m.out = reinterpret_cast<void*>(list[i].out);

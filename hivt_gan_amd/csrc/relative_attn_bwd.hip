@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restric
   T* const vt = kt + kBN * TL::PITCH;
   float* const bias = reinterpret_cast<float*>(vt + kBN * TL::PITCH);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   const int qtiles = (a.M + 64 * QB - 1) / (64 * QB);
   int unit, inner;
   walk(blockIdx.x, a.B * a.H, qtiles, unit, inner);
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
   float4* const rowst = reinterpret_cast<float4*>(ot + BQ * TL::PITCH);  // m, 1 / l, delta of a row
   float* const bias = reinterpret_cast<float*>(rowst + BQ);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   const int ktiles = (a.N + 64 * KB - 1) / (64 * KB);
   int unit, ktile;
   walk(blockIdx.x, a.B * a.G, ktiles, unit, ktile);
@@ -483,31 +483,44 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
     if (behind && from == 0) from = 1;  // distance 0 belongs to the other side
     float sum = 0.0f;
     for (int n = from; n < to; ++n) sum += diag[behind ? a.sat + n : a.sat - n];
-    partial[((int64_t)unit * groups + group) * a.buckets + bucket] = sum;
+    partial[(((int64_t)b * groups + group) * a.H + h) * a.buckets + bucket] = sum;
   }
 }
 
-// d_table[bucket][h] = the partial sums of head h, over batches and row groups in ascending order within each of the 16
-// slices a workgroup cuts them into, the slices in ascending order; in 64 bits.
-__global__ __launch_bounds__(1024) void table_kernel(const Args a, const float* __restrict__ partial, int groups,
+// d_table[bucket][h] = sum over the rows of partial [rows][H][buckets]: a workgroup takes 64 columns and cuts the rows into
+// 16 slices, each added in ascending order, then the slices; in 64 bits.
+__global__ __launch_bounds__(1024) void table_kernel(const float* __restrict__ partial, int64_t rows, int H, int buckets,
                                                      float* __restrict__ d_table) {
   __shared__ double sums[16][64];
-  const int h = blockIdx.x, bucket = blockIdx.y * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
-  const int64_t count = (int64_t)a.B * groups;
+  const int slice = threadIdx.x >> 6;
+  const int64_t cols = (int64_t)H * buckets, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
   double s = 0.0;
-  if (bucket < a.buckets) {
-    const int64_t end = count * (slice + 1) / 16;
-    for (int64_t i = count * slice / 16; i < end; ++i) {
-      const int64_t b = i / groups, grp = i % groups;
-      s += partial[((b * a.H + h) * groups + grp) * a.buckets + bucket];
+  if (col < cols) {
+    const int64_t end = rows * (slice + 1) / 16;
+    int64_t i = rows * slice / 16;
+    const float* p = partial + i * cols + col;
+    for (; i + 8 <= end; i += 8, p += 8 * cols) {  // eight loads on their way at once
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = p[j * cols];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
     }
+    for (; i < end; ++i, p += cols) s += *p;
   }
   sums[slice][threadIdx.x & 63] = s;
   __syncthreads();
-  if (slice == 0 && bucket < a.buckets) {
+  if (slice == 0 && col < cols) {
     for (int i = 1; i < 16; ++i) s += sums[i][threadIdx.x];
-    d_table[(int64_t)bucket * a.H + h] = (float)s;
+    d_table[col % buckets * H + col / buckets] = (float)s;
   }
+}
+int launch_table(const Args& a, const float* partial, int64_t rows, hipStream_t stream) {
+  const int64_t cols = (int64_t)a.H * a.buckets;
+  hipLaunchKernelGGL(table_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, stream, partial, rows, a.H, a.buckets,
+                     a.d_table);
+  HIVT_CHECK_LAUNCH("hivt_relative_attn_bwd");
+  return HIVT_OK;
 }
 
 constexpr int rows_per_group(int M) { return M <= 64 ? 16 : 32; }
@@ -518,6 +531,12 @@ struct Work {
 };
 Work work_of(const Args& a) {
   Work w;
+  if (short_bwd_route(a)) {
+    w.groups = short_slots(a);
+    w.delta = w.far = w.partial = 0;
+    w.total = a.want_table ? align_up((size_t)w.groups * a.H * a.buckets * sizeof(float), 256) : 0;
+    return w;
+  }
   w.groups = (a.M + rows_per_group(a.M) - 1) / rows_per_group(a.M);
   w.delta = 0;
   w.far = align_up((size_t)a.B * a.H * a.M * sizeof(float), 256);
@@ -550,9 +569,7 @@ int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
     hipLaunchKernelGGL((bias_kernel<T, DP, QB>), dim3((unsigned)((int64_t)a.B * a.H * w.groups)), dim3(64), lb, stream, a,
                        far_sums, partial);
     HIVT_CHECK_LAUNCH(what);
-    hipLaunchKernelGGL(table_kernel, dim3(a.H, (a.buckets + 63) / 64), dim3(1024), 0, stream, a, partial, w.groups,
-                       a.d_table);
-    HIVT_CHECK_LAUNCH(what);
+    return launch_table(a, partial, (int64_t)a.B * w.groups, stream);
   }
   return HIVT_OK;
 }
@@ -587,8 +604,6 @@ int launch_type(const Args& a, char* ws, const Work& w, hipStream_t stream) {
 
 }  // namespace
 
-int from_public(const char* what, const hivt_relative_attn* p, const int32_t* starts, float scale, Args& a);
-
 }  // namespace rel
 }  // namespace hivt
 
@@ -612,8 +627,13 @@ extern "C" int hivt_relative_attn_bwd(const hivt_relative_attn* p, const int32_t
   HIVT_REQUIRE(a.B == 0 || a.N == 0 || (a.k && a.v && a.dk && a.dv), HIVT_ERR_ARG, "%s: null pointer", what);
   HIVT_REQUIRE(a.B > 0 && a.M > 0, HIVT_ERR_ARG, "%s: no query rows: the gradients are zero", what);
   const Work w = work_of(a);
-  HIVT_REQUIRE(workspace != nullptr && workspace_bytes >= w.total, HIVT_ERR_WORKSPACE,
+  HIVT_REQUIRE(w.total == 0 || (workspace != nullptr && workspace_bytes >= w.total), HIVT_ERR_WORKSPACE,
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, w.total);
+  if (short_bwd_route(a)) {
+    float* const partial = a.want_table ? static_cast<float*>(workspace) : nullptr;
+    const int rs = short_bwd(a, (int)p->dtype, w.groups, partial, (hipStream_t)stream);
+    return rs == HIVT_OK && a.want_table ? launch_table(a, partial, w.groups, (hipStream_t)stream) : rs;
+  }
   char* const ws = static_cast<char*>(workspace);
   a.delta = reinterpret_cast<float*>(ws + w.delta);
   switch (p->dtype) {

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
   T* const vt = kt + kBN * TL::PITCH;
   float* const bias = reinterpret_cast<float*>(vt + kBN * TL::PITCH);
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   const int group = a.pack ? a.rep : 1;                    // heads whose rows share a tile
   const int rows = a.M * group;
   const int qtiles = (rows + 64 * QB - 1) / (64 * QB);
@@ -236,16 +236,31 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const int b = unit / heads, h = (unit % heads) * group + r % group, s = r / group;
   const float* const p0 = a.partial + ((int64_t)unit * a.splits * rows + r) * (a.d + 2);
   const int64_t step = (int64_t)rows * (a.d + 2);
-  float m = -INFINITY;
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, p0[i * step + a.d]);
+  // at most 128 splits: a lane weighs two of them
+  float ms[2], w[2], l = 0.0f, m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane + 64 * j;
+    ms[j] = i < a.splits ? p0[i * step + a.d] : -INFINITY;
+    w[j] = i < a.splits ? p0[i * step + a.d + 1] : 0.0f;
+    m = fmaxf(m, ms[j]);
+  }
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float m_safe = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float sum = w[j];
+    w[j] = fexp2(ms[j] - m_safe);
+    l += w[j] * sum;
+  }
+  l = wave_sum(l);
+  float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll 8
   for (int i = 0; i < a.splits; ++i) {
     const float* p = p0 + i * step;
-    const float w = fexp2(p[a.d] - m_safe);
-    l += w * p[a.d + 1];
-    if (lane < a.d) o0 += w * p[lane];
-    if (lane + 64 < a.d) o1 += w * p[lane + 64];
+    const float wi = __shfl(i < 64 ? w[0] : w[1], i & 63, 64);
+    if (lane < a.d) o0 += wi * p[lane];
+    if (lane + 64 < a.d) o1 += wi * p[lane + 64];
   }
   const float norm = l != l ? l : l > 0.0f ? 1.0f / l : 0.0f;
   T* out = static_cast<T*>(a.out) + b * a.o_st[0] + s * a.o_st[1] + h * a.o_st[2];
@@ -311,8 +326,6 @@ void plan(Args& a) {
 
 }  // namespace
 
-int from_public(const char* what, const hivt_relative_attn* p, const int32_t* starts, float scale, Args& a);
-
 }  // namespace rel
 }  // namespace hivt
 
@@ -326,6 +339,7 @@ static size_t split_bytes(const Args& a) {
 extern "C" size_t hivt_relative_attn_fwd_workspace_bytes(const hivt_relative_attn* p, const int32_t* starts) {
   Args a;
   if (from_public("hivt_relative_attn_fwd", p, starts, 1.0f, a) != HIVT_OK || a.B == 0 || a.M == 0) return 0;
+  if (short_fwd_route(a)) return 0;
   plan(a);
   return align_up(split_bytes(a), 256);
 }
@@ -336,11 +350,13 @@ extern "C" int hivt_relative_attn_fwd(const hivt_relative_attn* p, const int32_t
   Args a;
   const int rc = from_public(what, p, starts, scale, a);
   if (rc != HIVT_OK || a.B == 0 || a.M == 0) return rc;
-  plan(a);
+  const bool is_short = short_fwd_route(a);
+  if (!is_short) plan(a);
   const size_t need = split_bytes(a);
   HIVT_REQUIRE(a.q && a.table && a.out && (a.N == 0 || (a.k && a.v)), HIVT_ERR_ARG, "%s: null pointer", what);
   HIVT_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), HIVT_ERR_WORKSPACE,
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  if (is_short) return short_fwd(a, (int)p->dtype, (hipStream_t)stream);
   a.partial = static_cast<float*>(workspace);
   switch (p->dtype) {
     case HIVT_F32: return launch_type<float>(a, (hipStream_t)stream);

@@ -310,5 +310,15 @@ __device__ __forceinline__ void walk(int linear, int outer_count, int inner_coun
   }
 }
 
+// relative_attn_short.hip: which problems it takes, and its launches
+bool short_fwd_route(const Args& a);
+bool short_bwd_route(const Args& a);
+int short_slots(const Args& a);
+int short_fwd(const Args& a, int dtype, hipStream_t stream);
+int short_bwd(const Args& a, int dtype, int slots, float* partial, hipStream_t stream);
+
+// relative_attn_fwd.hip: the checked arguments of an entry point
+int from_public(const char* what, const hivt_relative_attn* p, const int32_t* starts, float scale, Args& a);
+
 }  // namespace rel
 }  // namespace hivt

@@ -244,8 +244,19 @@ __global__ __launch_bounds__(1024) void gain_kernel(const float* __restrict__ pa
   __shared__ double sums[16][64];
   const int col = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
   double s = 0.0;
-  if (col < 2 * d)
-    for (int r = rows * slice / 16; r < rows * (slice + 1) / 16; ++r) s += partial[(int64_t)r * 2 * d + col];
+  if (col < 2 * d) {
+    int r = rows * slice / 16;
+    const int end = rows * (slice + 1) / 16;
+    const float* p = partial + (int64_t)r * 2 * d + col;
+    for (; r + 8 <= end; r += 8, p += 16 * d) {  // eight loads on their way at once
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = p[j * 2 * d];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; r < end; ++r, p += 2 * d) s += *p;
+  }
   sums[slice][threadIdx.x & 63] = s;
   __syncthreads();
   if (slice == 0 && col < 2 * d) {
