@@ -7,11 +7,11 @@
 //   P = a + b G + c G^2,  Q <- P Q,  G <- P G P   per step, and X <- Q X once at the end of the phase.
 // With X m x n that costs 3 m^2 n per phase and 5 m^3 or fewer per step (symmetric products at half, only the tiles on and
 // below the diagonal are computed) instead of 3 m^2 n + m^3 per step.  A phase forms G from the rounded X of the phase
-// before: what the squares of small singular values lose in G comes back only there.  Hence the phases' lengths: 2 + 3
-// steps for n >= 1.5 m (23 instead of 27.5 m^3 at 1.5, 38 instead of 65 at 4); single steps for nearly square matrices,
-// where that costs the same (20 m^3) and is the most accurate (a 64 x 64 one with columns falling to 1e-3: 3e-7 off
-// instead of 4e-6).  One phase of five would save another third of a wide one, but is 5e-3 off on matrices of low rank,
-// even for 16-bit results too much.
+// before: what the squares of small singular values lose in G comes back only there.  Hence the phases' lengths: single
+// steps for nearly square matrices (n < 1.5 m), where that costs the same (20 m^3) and is the most accurate (a 64 x 64 one
+// with columns falling to 1e-3: 3e-7 off instead of 4e-6 with 2 + 3); else 1 + 2 + 2 for fp32 (47 instead of 65 m^3 at
+// n = 4 m) and 2 + 3 for 16-bit results (38 m^3; 128 x 20 of low rank: 3.0e-6 off, fp32 products by the definition 1.8e-6).
+// One phase of five would save more, but is 5e-3 off on matrices of low rank, even for 16-bit results too much.
 //
 // Bound by the matrix cores.  fp32 ones are eight times slower than 16-bit ones, so a value x is kept as two fp16 numbers
 // (hi = fp16(s x), lo = fp16(s x - hi)) and a product is hi hi + hi lo + lo hi with fp32 sums: 2^-24 of the value per
@@ -35,6 +35,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMats = 64;        // matrices per launch (descriptors travel in the argument block)
 constexpr int kPad = 64;
@@ -211,24 +212,30 @@ struct Product {
   float alpha, beta, diag;
 };
 
-template <int BM> struct Cfg {
-  static constexpr int BK = 32;
-  static constexpr int WT = BM / 2;        // a wave's square
-  static constexpr int NT = WT / 32;       // 32 x 32 blocks along it
-  static constexpr int TILE = BM / 64 * 2 * kBlock;   // halves of an operand's step in LDS
-  static constexpr int NPT = TILE * 2 / 16 / 256;     // 16-byte pieces of it per thread
+// A workgroup's square of results.  Its loop is bound by latency if nothing is done about it: a step of 32 takes 200 to
+// 800 clocks of matrix work and its operands, just written by another kernel, over 2000 to arrive.  So AHEAD steps are on
+// their way into registers (variables of their own: an indexed ring goes to scratch memory, which made the loop four
+// times slower) and two in LDS.
+template <int BM_> struct Cfg {
+  static constexpr int BM = BM_, BK = 32;
+  static constexpr int THREADS = BM == 256 ? 512 : 256;
+  static constexpr int AHEAD = BM == 64 ? 4 : BM == 128 ? 2 : 1;
+  static constexpr int WM = BM / (BM == 256 ? 4 : 2), WN = BM / 2;  // a wave's rows and columns
+  static constexpr int TM = WM / 32, TN = WN / 32;                  // 32 x 32 blocks of them
+  static constexpr int TILE = BM / 64 * 2 * kBlock;                 // halves of an operand's step in LDS
+  static constexpr int NPT = TILE * 2 / 16 / THREADS;               // 16-byte pieces of it per thread
 };
 
 template <int BM>
-__global__ __launch_bounds__(256) void product_kernel(const Group g, const Product p) {
+__global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g, const Product p) {
   using C = Cfg<BM>;
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][2][C::TILE];  // A, B; double-buffered
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds_all[];  // [2][A, B][TILE]
   const int gi = which(g, blockIdx.x);
   const Mat& mat = g.mats[gi];
   const Layout l = layout_of(mat.rows, mat.cols);
   char* const ws = g.base + mat.ws;
   const int block = blockIdx.x - g.first[gi];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float x0 = *reinterpret_cast<const float*>(ws);
 
   const bool apply = p.shape == SHAPE_APPLY, gram = p.shape == SHAPE_GRAM;
@@ -249,63 +256,113 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
   const _Float16* B = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : apply ? l.xt(p.from) : l.sq(p.b)));
   // (a 128-row tile may reach past an operand, which is padded to 64 rows: it reads the last block again and does not
   // store those results)
-  uint4 regs[2][C::NPT];
-  auto fetch = [&](int step) {
+  const int steps = K / C::BK;
+  struct Step { u32x4 a[C::NPT], b[C::NPT]; };
+  auto fetch = [&](Step& r, int step) {
+    step = min(step, steps - 1);
 #pragma unroll
     for (int i = 0; i < C::NPT; ++i) {
-      const int idx = tid + i * 256, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;  // block of 64 rows; halves
+      const int idx = tid + i * C::THREADS, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;
       const int64_t ra = (int64_t)min((i0 >> 6) + sub, (M >> 6) - 1) * (K >> 5) + step;
       const int64_t rb = (int64_t)min((j0 >> 6) + sub, (N >> 6) - 1) * (K >> 5) + step;
-      regs[0][i] = *reinterpret_cast<const uint4*>(A + ra * (2 * kBlock) + in);
-      regs[1][i] = *reinterpret_cast<const uint4*>(B + rb * (2 * kBlock) + in);
+      r.a[i] = *reinterpret_cast<const u32x4*>(A + ra * (2 * kBlock) + in);
+      r.b[i] = *reinterpret_cast<const u32x4*>(B + rb * (2 * kBlock) + in);
     }
   };
-  auto put = [&](int buf) {
+  auto put = [&](const Step& r, int buf) {
 #pragma unroll
-    for (int i = 0; i < C::NPT; ++i)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) *reinterpret_cast<uint4*>(&lds[buf][q][(tid + i * 256) * 8]) = regs[q][i];
+    for (int i = 0; i < C::NPT; ++i) {
+      _Float16* const at = lds_all + buf * 2 * C::TILE + (tid + i * C::THREADS) * 8;
+      *reinterpret_cast<u32x4*>(at) = r.a[i];
+      *reinterpret_cast<u32x4*>(at + C::TILE) = r.b[i];
+    }
   };
 
-  f32x16 acc[C::NT][C::NT];
+  f32x16 acc[C::TM][C::TN];
 #pragma unroll
-  for (int i = 0; i < C::NT; ++i)
+  for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-    for (int j = 0; j < C::NT; ++j)
+    for (int j = 0; j < C::TN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-  const int wi = (wave >> 1) * C::WT, wj = (wave & 1) * C::WT;
-
-  fetch(0);
-  put(0);
-  __syncthreads();
-  const int steps = K / C::BK;
-  for (int s = 0; s < steps; ++s) {
-    const int buf = s & 1;
-    if (s + 1 < steps) fetch(s + 1);
+  const int wi = (wave >> 1) * C::WM, wj = (wave & 1) * C::WN;
+  auto compute = [&](int buf) {
+    const _Float16* const la = lds_all + buf * 2 * C::TILE;
+    const _Float16* const lb = la + C::TILE;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      f16x8 fa[2][C::NT], fb[2][C::NT];
+      f16x8 fa[2][C::TM], fb[2][C::TN];
       const int piece = ks * 2 + (lane >> 5);
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int i = 0; i < C::NT; ++i) {
-          const int ra = wi + i * 32 + (lane & 31), rb = wj + i * 32 + (lane & 31);
-          fa[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][0][((ra >> 6) * 2 + q) * kBlock + lds_at(ra & 63, piece)]);
-          fb[q][i] = *reinterpret_cast<const f16x8*>(&lds[buf][1][((rb >> 6) * 2 + q) * kBlock + lds_at(rb & 63, piece)]);
+        for (int i = 0; i < C::TM; ++i) {
+          const int r = wi + i * 32 + (lane & 31);
+          fa[q][i] = *reinterpret_cast<const f16x8*>(la + ((r >> 6) * 2 + q) * kBlock + lds_at(r & 63, piece));
         }
 #pragma unroll
-      for (int i = 0; i < C::NT; ++i)
+        for (int j = 0; j < C::TN; ++j) {
+          const int r = wj + j * 32 + (lane & 31);
+          fb[q][j] = *reinterpret_cast<const f16x8*>(lb + ((r >> 6) * 2 + q) * kBlock + lds_at(r & 63, piece));
+        }
+      }
 #pragma unroll
-        for (int j = 0; j < C::NT; ++j) {
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
         }
     }
-    if (s + 1 < steps) put(buf ^ 1);  // (that buffer's readers passed the barrier of the step before)
+  };
+
+  // one step: its products, then the next one's operands into the other buffer (whose readers passed the barrier of the
+  // step before) and a later one's on their way.  The steps are an even number: sides are padded to 64.
+  auto turn = [&](int buf, Step& r, int later) {
+    compute(buf);
+    put(r, buf ^ 1);
+    fetch(r, later);
     __syncthreads();
+  };
+  if constexpr (C::AHEAD == 4) {
+    Step r0, r1, r2, r3;
+    fetch(r0, 0);
+    fetch(r1, 1);
+    fetch(r2, 2);
+    fetch(r3, 3);
+    put(r0, 0);
+    fetch(r0, 4);
+    __syncthreads();
+    for (int s = 0;; s += 4) {
+      turn(0, r1, s + 5);
+      turn(1, r2, s + 6);
+      if (s + 2 >= steps) break;
+      turn(0, r3, s + 7);
+      turn(1, r0, s + 8);
+      if (s + 4 >= steps) break;
+    }
+  } else if constexpr (C::AHEAD == 1) {  // (two would not fit the registers of two waves per SIMD)
+    Step r0;
+    fetch(r0, 0);
+    put(r0, 0);
+    fetch(r0, 1);
+    __syncthreads();
+    for (int s = 0; s < steps; s += 2) {
+      turn(0, r0, s + 2);
+      turn(1, r0, s + 3);
+    }
+  } else {
+    Step r0, r1;
+    fetch(r0, 0);
+    fetch(r1, 1);
+    put(r0, 0);
+    fetch(r0, 2);
+    __syncthreads();
+    for (int s = 0; s < steps; s += 2) {
+      turn(0, r1, s + 3);
+      turn(1, r0, s + 4);
+    }
   }
 
   // results: column = lane & 31, rows 8 (e / 4) + 4 (lane >> 5) + e % 4 of a 32 x 32 block
@@ -316,9 +373,9 @@ __global__ __launch_bounds__(256) void product_kernel(const Group g, const Produ
   const _Float16* R = p.r >= 0 ? reinterpret_cast<const _Float16*>(ws + l.sq(p.r)) : nullptr;
   const float rscale = ldexpf(p.beta, -p.er);
 #pragma unroll
-  for (int bi = 0; bi < C::NT; ++bi)
+  for (int bi = 0; bi < C::TM; ++bi)
 #pragma unroll
-    for (int bj = 0; bj < C::NT; ++bj)
+    for (int bj = 0; bj < C::TN; ++bj)
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int row = i0 + wi + bi * 32 + e4 * 8 + (lane >> 5) * 4, col = j0 + wj + bj * 32 + (lane & 31);
@@ -381,21 +438,35 @@ int64_t tiles_of(const Mat& a, int shape, int bm) {
   return shape == SHAPE_APPLY ? tm * tn : tm * (tm + 1) / 2;
 }
 
-int launch_product(Group& g, const Product& p, hipStream_t stream) {
+template <int BM>
+int launch_tiles(Group& g, const Product& p, hipStream_t stream) {
+  using C = Cfg<BM>;
   const char* what = "hivt_orthogonalize";
-  int64_t wide = 0;
-  for (int i = 0; i < g.count; ++i) wide += tiles_of(g.mats[i], p.shape, 128);
-  const int bm = wide >= 256 ? 128 : 64;  // the larger tile once it fills the compute units
   int64_t blocks = 0;
   for (int i = 0; i < g.count; ++i) {
     g.first[i] = (int32_t)blocks;
-    blocks += tiles_of(g.mats[i], p.shape, bm);
+    blocks += tiles_of(g.mats[i], p.shape, BM);
     HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
   }
-  if (bm == 128) hipLaunchKernelGGL(product_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, stream, g, p);
-  else hipLaunchKernelGGL(product_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, stream, g, p);
+  const size_t lds = (size_t)4 * C::TILE * sizeof(_Float16);
+  if (lds > 48 * 1024)
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<BM>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
+  hipLaunchKernelGGL(product_kernel<BM>, dim3((unsigned)blocks), dim3(C::THREADS), lds, stream, g, p);
   HIVT_CHECK_LAUNCH(what);
   return HIVT_OK;
+}
+
+// The largest tile that still gives every compute unit one.
+int launch_product(Group& g, const Product& p, hipStream_t stream) {
+  int64_t at256 = 0, at128 = 0;
+  for (int i = 0; i < g.count; ++i) {
+    at256 += tiles_of(g.mats[i], p.shape, 256);
+    at128 += tiles_of(g.mats[i], p.shape, 128);
+  }
+  if (at256 >= 256) return launch_tiles<256>(g, p, stream);
+  if (at128 >= 256) return launch_tiles<128>(g, p, stream);
+  return launch_tiles<64>(g, p, stream);
 }
 
 // exponent of the scale of a product of k factors P (each at most 3.45)
@@ -506,11 +577,11 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   for (int32_t i = 0; i < count; ++i)
     HIVT_REQUIRE(list[i].rows * list[i].cols == 0 || (list[i].in && list[i].out), HIVT_ERR_ARG, "%s: null pointer", what);
-  // two kinds of matrices: nearly square ones, and wide ones with phases of up to three steps
+  // two kinds of matrices: nearly square ones, and wide ones with phases of up to two or three
   int64_t at = 0;
   for (int kind = 0; kind < 2; ++kind) {
     int phases[16], n = 0, left = steps;
-    const int most = kind == 0 ? 1 : 3;
+    const int most = kind == 0 ? 1 : dtype == HIVT_F32 ? 2 : 3;
     if (left % most != 0) { phases[n++] = left % most; left -= left % most; }
     for (; left > 0; left -= most) phases[n++] = most;
     Group g;
