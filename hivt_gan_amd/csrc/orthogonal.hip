@@ -88,6 +88,8 @@ __device__ __forceinline__ int which(const Group& g, int block) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < g.count && g.first[lane] <= block)) - 1);
 }
 
+__host__ __device__ inline bool is_wide(int64_t rows, int64_t cols) { return 2 * rows >= 3 * cols || 2 * cols >= 3 * rows; }
+
 __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
   if (dtype == HIVT_F32) return static_cast<const float*>(p)[i];
   if (dtype == HIVT_BF16) return (float)static_cast<const __bf16*>(p)[i];
@@ -432,6 +434,291 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
       }
 }
 
+// ---- small matrices: all steps in one workgroup ---------------------------------------------------------------------------
+// With the smaller side at most 128 a product is a few microseconds of one compute unit, less than the launch in between:
+// a workgroup takes a matrix through all phases.  G and the polynomials stay in LDS (two square operands: a phase has at
+// most two steps), X comes through a staging buffer of 32 of the reduction index and goes back to the workspace.  A result
+// is symmetric, or wanted transposed as well, so four consecutive rows of a lane are stored as one piece of a row.
+// 62 matrices of the 128-wide model: 2 + 1 launches instead of 37.
+template <int MP> struct Small {
+  static constexpr int THREADS = MP == 128 ? 512 : 256;
+  static constexpr int TN = MP / 64;                        // 32 x 32 blocks of a wave along the columns (one along the rows)
+  static constexpr int SQUARE = MP * MP * 2;                // halves of a square operand
+  static constexpr int STAGE = MP * 32 * 2;                 // halves of a staged step
+  static constexpr int NPT = STAGE * 2 / 16 / THREADS;
+  static constexpr size_t LDS = (size_t)(2 * SQUARE + STAGE) * sizeof(_Float16);
+};
+
+template <int MP>
+__global__ __launch_bounds__(Small<MP>::THREADS) void small_kernel(const Group g, int steps_wanted) {
+  using C = Small<MP>;
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds_all[];
+  _Float16* const s0 = lds_all;
+  _Float16* const s1 = s0 + C::SQUARE;
+  _Float16* const stage = s1 + C::SQUARE;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Mat& mat = g.mats[blockIdx.x];
+  const Layout l = layout_of(mat.rows, mat.cols);
+  char* const ws = g.base + mat.ws;
+  const float x0 = *reinterpret_cast<const float*>(ws);
+  _Float16* const X = reinterpret_cast<_Float16*>(ws + l.x);
+  _Float16* const Xt = reinterpret_cast<_Float16*>(ws + l.xt(0));
+  const int wi = (wave >> 1) * 32, wj = (wave & 1) * (MP / 2);
+  const int mb = l.mp >> 6;  // blocks of 64 rows that exist (1 or 2)
+
+  f32x16 acc[C::TN], turned[C::TN];
+  auto clear = [&](f32x16 (&acc)[C::TN]) {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][e] = 0.0f;
+  };
+  // 32 of the reduction index: A and B in blocks, `stride` blocks apart per 64 rows
+  auto multiply = [&](f32x16 (&acc)[C::TN], const _Float16* A, int sa, const _Float16* B, int sb) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int piece = ks * 2 + (lane >> 5);
+      const int ra = wi + (lane & 31);
+      f16x8 fa[2], fb[2][C::TN];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        fa[q] = *reinterpret_cast<const f16x8*>(A + ((ra >> 6) * sa * 2 + q) * kBlock + lds_at(ra & 63, piece));
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+          const int rb = wj + j * 32 + (lane & 31);
+          fb[q][j] = *reinterpret_cast<const f16x8*>(B + ((rb >> 6) * sb * 2 + q) * kBlock + lds_at(rb & 63, piece));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j) {
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[0][j], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[1][j], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1], fb[0][j], acc[j], 0, 0, 0);
+      }
+    }
+  };
+  constexpr int KB = MP / 32;  // steps of a square operand
+  auto square = [&](const _Float16* A, const _Float16* B) {
+    clear(acc);
+#pragma unroll 1
+    for (int kb = 0; kb < KB; ++kb) multiply(acc, A + kb * 2 * kBlock, KB, B + kb * 2 * kBlock, KB);
+  };
+  // the lane's number, anew: offsets that the compiler would otherwise hold over all phases, for want of registers in memory
+  auto anew = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  // acc * 2^-down (+ b G + a I) as a square operand of scale 2^ed; G: the operand it was made from (scale 2^14)
+  auto keep = [&](_Float16* dst, int down, int ed, float alpha, const _Float16* G) {
+    const float unscale = ldexpf(alpha, -down), gscale = ldexpf(kB, -14);
+    const int ln = anew(lane);
+    float v[C::TN][16];
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int row = wi + e4 * 8 + (ln >> 5) * 4, col = wj + j * 32 + (ln & 31);
+        f16x4 gh, gl;
+        if (G != nullptr) {  // (symmetric: row `col`, four columns)
+          const int64_t at = at_of(col, row, MP);
+          gh = *reinterpret_cast<const f16x4*>(G + at);
+          gl = *reinterpret_cast<const f16x4*>(G + at + kBlock);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = acc[j][e4 * 4 + e] * unscale;
+          if (G != nullptr) {
+            x += gscale * ((float)gh[e] + (float)gl[e]);
+            if (row + e == col) x += kA;
+          }
+          v[j][e4 * 4 + e] = row + e < l.m && col < l.m ? ldexpf(x, ed) : 0.0f;
+        }
+      }
+    __syncthreads();  // every wave has read its operands
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int row = wi + e4 * 8 + (ln >> 5) * 4, col = wj + j * 32 + (ln & 31);
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          _Float16 h, o;
+          split(v[j][e4 * 4 + e], h, o);
+          hi[e] = h;
+          lo[e] = o;
+        }
+        const int64_t at = at_of(col, row, MP);
+        *reinterpret_cast<f16x4*>(dst + at) = hi;
+        *reinterpret_cast<f16x4*>(dst + at + kBlock) = lo;
+      }
+    __syncthreads();
+  };
+  // a step of a staged operand: `blocks` blocks of 64 rows from `src` on, `stride` blocks apart; rows that are not there
+  // repeat the last
+  struct Step { u32x4 r[C::NPT]; };
+  Step r0, r1, r2, r3;  // four steps on their way: a step computes a tenth of the time that its operands take to arrive
+  auto fetch = [&](Step& r, const _Float16* src, int stride, int blocks) {
+    const int id = anew(tid);
+#pragma unroll
+    for (int i = 0; i < C::NPT; ++i) {
+      const int idx = id + i * C::THREADS, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;
+      r.r[i] = *reinterpret_cast<const u32x4*>(src + (int64_t)min(sub, blocks - 1) * stride * (2 * kBlock) + in);
+    }
+  };
+  auto put = [&](const Step& r) {
+#pragma unroll
+    for (int i = 0; i < C::NPT; ++i) *reinterpret_cast<u32x4*>(stage + (tid + i * C::THREADS) * 8) = r.r[i];
+  };
+
+  const int kn = l.np >> 5, km = l.mp >> 5, nb = l.np >> 6;
+  constexpr int CB = MP / 64;  // blocks of 64 columns of X at a time
+  auto fetch_x = [&](Step& r, int k) { fetch(r, X + (int64_t)min(k, kn - 1) * 2 * kBlock, kn, mb); };
+  auto fetch_xt = [&](Step& r, int c, int k) {
+    c = min(c, nb - 1);
+    fetch(r, Xt + ((int64_t)c * km + min(k, km - 1)) * 2 * kBlock, km, min(CB, nb - c));
+  };
+
+  const int at_once = is_wide(mat.rows, mat.cols) ? 2 : 1;
+  int taken = 0;
+  while (taken < steps_wanted) {
+    const int steps = (steps_wanted - taken) % at_once != 0 ? 1 : at_once;
+    const bool last = taken + steps == steps_wanted;
+    const int ex = x_exponent(x0, taken), ex_after = x_exponent(x0, taken + steps);
+    // G = X X'
+    clear(acc);
+    fetch_x(r0, 0);
+    fetch_x(r1, 1);
+    fetch_x(r2, 2);
+    fetch_x(r3, 3);
+    auto gram = [&](Step& r, int later) {
+      __syncthreads();
+      put(r);
+      fetch_x(r, later);
+      __syncthreads();
+      multiply(acc, stage, 1, stage, 1);
+    };
+    for (int k = 0;; k += 4) {  // (an even number of steps)
+      gram(r0, k + 4);
+      gram(r1, k + 5);
+      if (k + 2 >= kn) break;
+      gram(r2, k + 6);
+      gram(r3, k + 7);
+      if (k + 4 >= kn) break;
+    }
+    fetch_xt(r0, 0, 0);
+    fetch_xt(r1, 0, 1);
+    fetch_xt(r2, 0, 2);
+    fetch_xt(r3, 0, 3);
+    keep(s0, 2 * ex, 14, 1.0f, nullptr);
+    // the polynomial in front of X: into s0
+    int eq = 14;
+    if (steps == 1) {
+      square(s0, s0);
+      keep(s0, 28, 14, kC, s0);
+    } else {
+      square(s0, s0);
+      keep(s1, 28, 14, kC, s0);      // P
+      square(s1, s0);
+      keep(s0, 28, 14, 1.0f, nullptr);  // P G
+      square(s0, s1);
+      keep(s0, 28, 14, 1.0f, nullptr);  // P G P
+      square(s0, s0);
+      keep(s0, 28, 14, kC, s0);      // the second P
+      square(s0, s1);
+      eq = 12;
+      keep(s0, 28, eq, 1.0f, nullptr);
+    }
+    // X <- Q X, MP columns at a time.  Both the result and its transpose are stored with the reduction index of a later
+    // product innermost, four of which a lane holds in a row only in the product with the operands exchanged: it is
+    // computed twice.  Pieces of 8 bytes go to 64 cache lines a store (13 000 clocks for 128 x 128); they are put together
+    // in LDS, in the free square operand, and leave it in whole lines.
+    const float unscale = ldexpf(1.0f, -(eq + ex));
+    for (int c = 0; c < nb; c += CB) {
+      clear(acc);
+      clear(turned);
+      auto apply = [&](Step& r, int k) {
+        __syncthreads();
+        put(r);
+        fetch_xt(r, c + CB, k);
+        __syncthreads();
+        multiply(acc, s0 + k * 2 * kBlock, KB, stage, 1);
+        if (!last) multiply(turned, stage, 1, s0 + k * 2 * kBlock, KB);
+      };
+      apply(r0, 0);
+      apply(r1, 1);
+      if (km == 4) {
+        apply(r2, 2);
+        apply(r3, 3);
+      }
+      // (these columns of Xt have been read; the rest of them belongs to other columns of X)
+      const int ln = anew(lane);
+      if (last) {
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int row = wi + (e >> 2) * 8 + (ln >> 5) * 4 + (e & 3), col = c * 64 + wj + j * 32 + (ln & 31);
+            if (row >= l.m || col >= l.n) continue;
+            const float x = acc[j][e] * unscale;
+            const int64_t at = mat.rows > mat.cols ? (int64_t)col * l.m + row : (int64_t)row * l.n + col;
+            if (g.dtype == HIVT_F32) static_cast<float*>(mat.out)[at] = x;
+            else if (g.dtype == HIVT_BF16) static_cast<__bf16*>(mat.out)[at] = (__bf16)x;
+            else static_cast<_Float16*>(mat.out)[at] = (_Float16)x;
+          }
+        continue;
+      }
+      // four elements of row `to` from element `from` on, into the image of a square operand
+      auto piece = [&](int to, int from, const f32x16& v, int e4, bool in, int limit) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          _Float16 h, o;
+          split(in && from + e < limit ? ldexpf(v[e4 * 4 + e] * unscale, ex_after) : 0.0f, h, o);
+          hi[e] = h;
+          lo[e] = o;
+        }
+        const int64_t at = at_of(to, from, MP);
+        *reinterpret_cast<f16x4*>(s1 + at) = hi;
+        *reinterpret_cast<f16x4*>(s1 + at + kBlock) = lo;
+      };
+      // blocks [rows][steps] of the image to memory, `stride` blocks apart per 64 rows
+      auto leave = [&](_Float16* dst, int rows, int steps, int stride) {
+        const int id = anew(tid);
+        for (int i = id; i < MP / 64 * KB * (2 * kBlock / 8); i += C::THREADS) {
+          const int block = i / (2 * kBlock / 8), in = i % (2 * kBlock / 8) * 8, rb = block / KB, kb = block % KB;
+          if (rb < rows && kb < steps)
+            *reinterpret_cast<u32x4*>(dst + ((int64_t)rb * stride + kb) * (2 * kBlock) + in) =
+                *reinterpret_cast<const u32x4*>(s1 + block * 2 * kBlock + in);
+        }
+      };
+      const int there = min(CB, nb - c);  // blocks of 64 columns
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {  // rows of X down, columns across
+          const int down = wi + e4 * 8 + (ln >> 5) * 4, across = wj + j * 32 + (ln & 31);
+          piece(across, down, acc[j], e4, c * 64 + across < l.n, l.m);
+        }
+      __syncthreads();
+      leave(Xt + (int64_t)c * km * 2 * kBlock, there, km, km);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {  // columns of X down, rows across
+          const int down = wi + e4 * 8 + (ln >> 5) * 4, across = wj + j * 32 + (ln & 31);
+          piece(across, down, turned[j], e4, across < l.m, l.n - c * 64);
+        }
+      __syncthreads();
+      leave(X + (int64_t)c * 2 * 2 * kBlock, mb, there * 2, kn);
+    }
+    taken += steps;
+    __threadfence();  // what this workgroup wrote to memory it reads again
+    __syncthreads();
+  }
+}
+
 int64_t tiles_of(const Mat& a, int shape, int bm) {
   const Layout l = layout_of(a.rows, a.cols);
   const int64_t tm = (l.mp + bm - 1) / bm, tn = (l.np + bm - 1) / bm;
@@ -472,8 +759,31 @@ int launch_product(Group& g, const Product& p, hipStream_t stream) {
 // exponent of the scale of a product of k factors P (each at most 3.45)
 int q_exponent(int k) { return 16 - 2 * k; }
 
-int run_group(Group& g, const int* phases, int nphases, hipStream_t stream) {
+template <int MP>
+int launch_small(const Group& g, int steps, hipStream_t stream) {
+  using C = Small<MP>;
   const char* what = "hivt_orthogonalize";
+  if (C::LDS > 48 * 1024)
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&small_kernel<MP>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS), what);
+  hipLaunchKernelGGL(small_kernel<MP>, dim3((unsigned)g.count), dim3(C::THREADS), C::LDS, stream, g, steps);
+  HIVT_CHECK_LAUNCH(what);
+  return HIVT_OK;
+}
+
+struct Phases { int32_t count, steps[16]; };
+
+// one workgroup to a matrix of this shape: 0 (no), or the smaller side that its kernel is made for
+int small_side(int64_t rows, int64_t cols) {
+  const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return m > 128 || n > 1024 ? 0 : m > 64 ? 128 : 64;
+}
+
+// small: one workgroup to a matrix, through all steps
+int run_group(Group& g, const Phases& list, bool small, int steps, hipStream_t stream) {
+  const char* what = "hivt_orthogonalize";
+  const int32_t* const phases = list.steps;
+  const int nphases = list.count;
   int64_t blocks = 0;
   for (int i = 0; i < g.count; ++i) {
     g.first[i] = (int32_t)blocks;
@@ -492,6 +802,12 @@ int run_group(Group& g, const int* phases, int nphases, hipStream_t stream) {
   hipLaunchKernelGGL(convert_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, g);
   HIVT_CHECK_LAUNCH(what);
 
+  if (small) {
+    // (a matrix of up to 64 gives the same bits in either kernel: the larger one adds zeros)
+    int side = 0;
+    for (int i = 0; i < g.count; ++i) side = max(side, small_side(g.mats[i].rows, g.mats[i].cols));
+    return side == 64 ? launch_small<64>(g, steps, stream) : launch_small<128>(g, steps, stream);
+  }
   int taken = 0, at = 0;
   for (int f = 0; f < nphases; ++f) {
     // square planes: 0 G, 1 P G, 2 P, and 3 / 4 in turn Q
@@ -577,13 +893,15 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
                "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   for (int32_t i = 0; i < count; ++i)
     HIVT_REQUIRE(list[i].rows * list[i].cols == 0 || (list[i].in && list[i].out), HIVT_ERR_ARG, "%s: null pointer", what);
-  // two kinds of matrices: nearly square ones, and wide ones with phases of up to two or three
+  // nearly square matrices, wide ones (with phases of up to two or three steps), small ones
   int64_t at = 0;
-  for (int kind = 0; kind < 2; ++kind) {
-    int phases[16], n = 0, left = steps;
+  for (int kind = 0; kind < 3; ++kind) {
+    Phases phases;
+    phases.count = 0;
+    int left = steps;
     const int most = kind == 0 ? 1 : dtype == HIVT_F32 ? 2 : 3;
-    if (left % most != 0) { phases[n++] = left % most; left -= left % most; }
-    for (; left > 0; left -= most) phases[n++] = most;
+    if (left % most != 0) { phases.steps[phases.count++] = left % most; left -= left % most; }
+    for (; left > 0; left -= most) phases.steps[phases.count++] = most;
     Group g;
     memset(&g, 0, sizeof(g));
     g.dtype = dtype;
@@ -593,7 +911,7 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
       if (i < count) {
         const int64_t r = list[i].rows, c = list[i].cols;
         if (r * c == 0) continue;
-        if ((2 * r >= 3 * c || 2 * c >= 3 * r) != (kind == 1)) continue;
+        if ((small_side(r, c) ? 2 : is_wide(r, c) ? 1 : 0) != kind) continue;
         Mat& m = g.mats[g.count++];
         m.in = reinterpret_cast<const void*>(list[i].in);
         m.out = reinterpret_cast<void*>(list[i].out);
@@ -603,7 +921,7 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
         at += layout_of(m.rows, m.cols).total;
       }
       if (g.count > 0 && (i == count || g.count == kMats)) {
-        rc = run_group(g, phases, n, (hipStream_t)stream);
+        rc = run_group(g, phases, kind == 2, steps, (hipStream_t)stream);
         if (rc != HIVT_OK) return rc;
         g.count = 0;
       }

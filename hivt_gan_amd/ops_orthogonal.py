@@ -21,6 +21,20 @@ def matrix_list(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor]):
     return (ctypes.c_int64 * max(1, len(flat)))(*flat)
 
 
+def _outputs(matrices: Sequence[torch.Tensor]) -> List[torch.Tensor]:
+    """A tensor like each matrix; those of one shape are slices of one allocation (a call of the allocator costs as much
+    as launching a kernel)."""
+    by_shape = {}
+    for i, x in enumerate(matrices):
+        by_shape.setdefault(x.shape, []).append(i)
+    out: List[Optional[torch.Tensor]] = [None] * len(matrices)
+    for shape, at in by_shape.items():
+        x = matrices[at[0]]
+        for i, y in zip(at, torch.empty((len(at), *shape), dtype=x.dtype, device=x.device).unbind(0)):
+            out[i] = y
+    return out
+
+
 @torch.no_grad()
 def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float = 1e-7,
                   out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
@@ -28,7 +42,8 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float =
     ``steps`` times ``x <- a x + (b g + c g^2) x`` with g = x x^T (of the shorter side) and a, b, c = 3.4445, -4.7750,
     2.0315.  One type for the list, float32, bfloat16 or float16; any shapes up to 65536 a side.  The arithmetic is that of
     fp32 whatever the type, rounded once at the end; results are the same whatever else is in the list.  ``out``:
-    contiguous tensors to write to (the matrices themselves are allowed).  Not differentiable."""
+    contiguous tensors to write to (the matrices themselves are allowed); without it, results of one shape are slices of one
+    allocation.  Not differentiable."""
     matrices = list(matrices)
     if not matrices:
         return []
@@ -48,7 +63,7 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float =
         raise ValueError(f"eps must be positive, got {eps}")
     _need_gpu(*matrices)
     if out is None:
-        out = [torch.empty(x.shape, dtype=dtype, device=device) for x in matrices]
+        out = _outputs(matrices)
     else:
         out = list(out)
         if len(out) != len(matrices):
