@@ -27,8 +27,9 @@ __device__ __forceinline__ float dot(const Frag<T, E>& a, const Frag<T, E>& b) {
   return s;
 }
 
+// Waves to a SIMD: two where the registers allow, so that one's matrix instructions run beside the other's exponentials.
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restrict__ far_sums) {
+__global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2) : DP <= (sizeof(T) == 4 ? 32 : 96) ? 2 : 1) void dq_kernel(const Args a, float2* __restrict__ far_sums) {
   using TL = Tile<T, DP>;
   constexpr int NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -98,8 +99,8 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restric
     if (t < t_end) {
       const int64_t k0 = (int64_t)t * kBN;
       auto keep = [&](int row) { return (bits >> row & 1) != 0; };
-      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, keep);
-      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, keep);
+      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, bits == ~0ull, keep);
+      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, bits == ~0ull, keep);
     }
   };
   seek();
@@ -117,6 +118,8 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restric
     const int rel_hi = k0 + kBN - 1 - pos_lo, rel_lo = k0 - pos_hi;
     const bool left = rel_hi <= -a.sat, right = rel_lo >= hi, far = left || right;
     const bool whole = keys == ~0ull && (!a.causal || rel_hi <= 0);
+    const float c = bias[left ? 0 : width - 1];
+    const bool plain = far && whole && fabsf(c) <= kPlainBias;  // (see the forward)
     // two 16-key blocks at a time: what the reduction over the keys takes
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -138,24 +141,35 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restric
       Frag<T, 8> df[QB];
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        const int rel0 = k0 + kk * 32 + quad * 4 - pos[qb] + a.sat;
-        const int lim = a.causal ? pos[qb] - k0 : kBN;
-        const float c = bias[left ? 0 : width - 1];
-        float sum_ds = 0.0f, sum_p = 0.0f;
+        float mul = a.scale2, add = c;  // (see the forward)
+        if (!plain) {
+          mul = 1.0f;
+          add = 0.0f;
+          const int rel0 = k0 + kk * 32 + quad * 4 - pos[qb] + a.sat;
+          const int lim = a.causal ? pos[qb] - k0 : kBN;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float add = far ? c : bias[min(max(rel0 + i * 16 + r, 0), width - 1)];
-            float p = fexp2(fmaf(s[i][qb][r], a.scale2, add) - m[qb]) * il[qb];
-            if (!whole && (!(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim)) p = dp[i][qb][r] = 0.0f;
-            const float ds = p * (dp[i][qb][r] - delta[qb]);
-            dp[i][qb][r] = ds;
-            sum_ds += ds;
-            sum_p += p;
+            for (int r = 0; r < 4; ++r) {
+              const float x = fmaf(s[i][qb][r], a.scale2, bias[min(max(rel0 + i * 16 + r, 0), width - 1)]);
+              const bool out = !(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim;
+              s[i][qb][r] = out ? -INFINITY : x;
+              dp[i][qb][r] = out ? 0.0f : dp[i][qb][r];
+            }
           }
         }
+        const float shift = add - m[qb];
+        float sum_ds = 0.0f, sum_p = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = fexp2(fmaf(s[i][qb][r], mul, shift)) * il[qb];
+            dp[i][qb][r] = p * (dp[i][qb][r] - delta[qb]);
+            sum_ds += dp[i][qb][r];
+            sum_p += p;
+          }
         rsum[qb] += sum_ds;
         if (left) { far_l[qb] += sum_ds; w_l[qb] += sum_p; }
         else if (right) { far_r[qb] += sum_ds; w_r[qb] += sum_p; }
@@ -197,9 +211,9 @@ __global__ __launch_bounds__(256) void dq_kernel(const Args a, float2* __restric
   }
 }
 
-// BQ query rows a step; a wave owns 16 KB keys.
-template <typename T, int DP, int KB, int BQ>
-__global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
+// BQ query rows a step; a wave owns 16 KB keys, a workgroup has WAVES of them.
+template <typename T, int DP, int KB, int BQ, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -209,13 +223,17 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
   float* const bias = reinterpret_cast<float*>(rowst + BQ);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
-  const int ktiles = (a.N + 64 * KB - 1) / (64 * KB);
-  int unit, ktile;
-  walk(blockIdx.x, a.B * a.G, ktiles, unit, ktile);
+  const int ktiles = (a.N + 16 * WAVES * KB - 1) / (16 * WAVES * KB);
+  // One query head to a workgroup, or (a.splits == 1) all of the group: their shares of dk and dv are then added by
+  // another kernel.
+  const int parts = a.splits, heads = a.rep / parts;
+  int unit, inner;
+  walk(blockIdx.x, a.B * a.G, ktiles * parts, unit, inner);
+  const int ktile = inner / parts, part = inner % parts;
   const int b = unit / a.G, g = unit % a.G;
   const int width = bias_width(a), hi = bias_hi(a);
 
-  const int key0 = ktile * 64 * KB + wave * 16 * KB;
+  const int key0 = ktile * 16 * WAVES * KB + wave * 16 * KB;
   bool keep[KB];
   int key[KB];
   Frag<T, TL::E> kf[KB][TL::KSTEPS], vf[KB][TL::KSTEPS];
@@ -249,12 +267,12 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
     for (int kb = 0; kb < KB; ++kb) dk[n][kb] = dv[n][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int qsteps = (a.M + BQ - 1) / BQ;
-  const int first = a.causal ? max(0, ktile * 64 * KB - a.offset) / BQ : 0;  // rows before it see none of these keys
-  Loader<T, DP, BQ, 256> ql, ol;
-  for (int hr = 0; hr < a.rep; ++hr) {
-    const int h = g * a.rep + hr;
+  const int first = a.causal ? max(0, ktile * 16 * WAVES * KB - a.offset) / BQ : 0;  // rows before it see none of these keys
+  Loader<T, DP, BQ, 64 * WAVES> ql, ol;
+  for (int hr = 0; hr < heads; ++hr) {
+    const int h = g * a.rep + part * heads + hr;
     __syncthreads();  // the head before has been finished by every wave
-    for (int e = tid; e < width; e += 256) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+    for (int e = tid; e < width; e += 64 * WAVES) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
     const T* const qbase = static_cast<const T*>(a.q) + b * a.q_st[0] + h * a.q_st[2];
     const T* const obase = static_cast<const T*>(a.d_out) + b * a.do_st[0] + h * a.do_st[2];
     const int64_t rowbase = ((int64_t)b * a.H + h) * a.M;
@@ -262,8 +280,8 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
     auto fetch = [&](int step) {
       const int s0 = step * BQ;
       auto in = [&](int row) { return s0 + row < a.M; };
-      ql.load(qbase + (int64_t)s0 * a.q_st[1], a.q_st[1], a.d, a.q_align, tid, in);
-      ol.load(obase + (int64_t)s0 * a.do_st[1], a.do_st[1], a.d, a.do_align, tid, in);
+      ql.load(qbase + (int64_t)s0 * a.q_st[1], a.q_st[1], a.d, a.q_align, tid, s0 + BQ <= a.M, in);
+      ol.load(obase + (int64_t)s0 * a.do_st[1], a.do_st[1], a.d, a.do_align, tid, s0 + BQ <= a.M, in);
       if (tid < BQ) {
         st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (s0 + tid < a.M) {
@@ -287,6 +305,7 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
       const bool left = rel_hi <= -a.sat, far = left || rel_lo >= hi;
       const bool whole = all && s0 + BQ <= a.M && (!a.causal || rel_hi <= 0);
       const float c = bias[left ? 0 : width - 1];
+      const bool plain = far && whole && fabsf(c) <= kPlainBias;  // (see the forward)
 #pragma unroll
       for (int qq = 0; qq < BQ / 32; ++qq) {
         f32x4 p[2][KB], ds[2][KB];
@@ -304,23 +323,41 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
             }
           }
         }
+        // (two ways with registers moved between them: put together as in the other kernels, the rows' statistics are read
+        // twice, which cost more: 122 -> 149 us for the encoder layer of 1024 positions)
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = qq * 32 + i * 16 + quad * 4 + r;
-            const float4 rs = rowst[row];
+            for (int r = 0; r < 4; ++r) {
+              const float4 rs = rowst[qq * 32 + i * 16 + quad * 4 + r];
+              const float shift = c - rs.x;
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-              const int rel = key[kb] - pos0 - row;
-              const float add = far ? c : bias[min(max(rel + a.sat, 0), width - 1)];
-              float w = fexp2(fmaf(p[i][kb][r], a.scale2, add) - rs.x) * rs.y;
-              float dp = ds[i][kb][r];
-              if (!whole && (!keep[kb] || s0 + row >= a.M || (a.causal && rel > 0))) w = dp = 0.0f;
-              p[i][kb][r] = w;
-              ds[i][kb][r] = w * (dp - rs.z);
+              for (int kb = 0; kb < KB; ++kb) {
+                const float w = fexp2(fmaf(p[i][kb][r], a.scale2, shift)) * rs.y;
+                p[i][kb][r] = w;
+                ds[i][kb][r] = w * (ds[i][kb][r] - rs.z);
+              }
             }
-          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int row = qq * 32 + i * 16 + quad * 4 + r;
+              const float4 rs = rowst[row];
+#pragma unroll
+              for (int kb = 0; kb < KB; ++kb) {
+                const int rel = key[kb] - pos0 - row;
+                const float add = bias[min(max(rel + a.sat, 0), width - 1)];
+                float w = fexp2(fmaf(p[i][kb][r], a.scale2, add) - rs.x) * rs.y;
+                float dp = ds[i][kb][r];
+                if (!keep[kb] || s0 + row >= a.M || (a.causal && rel > 0)) w = dp = 0.0f;
+                p[i][kb][r] = w;
+                ds[i][kb][r] = w * (dp - rs.z);
+              }
+            }
+        }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           const Frag<T, 8> pf = pair_frag<T>(p[0][kb], p[1][kb]), df = pair_frag<T>(ds[0][kb], ds[1][kb]);
@@ -336,6 +373,20 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     if (key[kb] >= a.N) continue;
+    if (parts > 1) {  // [part][batch, key, key head][dk, dv][d]
+      float* const share = a.partial + ((((int64_t)part * a.B + b) * a.N + key[kb]) * a.G + g) * 2 * a.d;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        f32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = keep[kb] ? dk[n][kb][j] * a.scale : 0.0f;
+        store4(share, n * 16 + quad * 4, a.d, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = keep[kb] ? dv[n][kb][j] : 0.0f;
+        store4(share + a.d, n * 16 + quad * 4, a.d, w);
+      }
+      continue;
+    }
     T* ok = static_cast<T*>(a.dk) + b * a.dk_st[0] + key[kb] * a.dk_st[1] + g * a.dk_st[2];
     T* ov = static_cast<T*>(a.dv) + b * a.dv_st[0] + key[kb] * a.dv_st[1] + g * a.dv_st[2];
 #pragma unroll
@@ -348,6 +399,21 @@ __global__ __launch_bounds__(256) void dkv_kernel(const Args a) {
       for (int j = 0; j < 4; ++j) w[j] = keep[kb] ? dv[n][kb][j] : 0.0f;
       store4(ov, n * 16 + quad * 4, a.d, w);
     }
+  }
+}
+
+// dk, dv = the sums of the query heads' shares, in ascending order of the heads
+template <typename T>
+__global__ __launch_bounds__(256) void group_kernel(const Args a) {
+  const int64_t rows = (int64_t)a.B * a.N * a.G, total = rows * 2 * a.d;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+    for (int p = 0; p < a.splits; ++p) s += a.partial[p * total + i];
+    const int64_t row = i / (2 * a.d);
+    const int c = (int)(i % (2 * a.d)), g = (int)(row % a.G);
+    const int64_t key = row / a.G % a.N, b = row / a.G / a.N;
+    if (c < a.d) static_cast<T*>(a.dk)[b * a.dk_st[0] + key * a.dk_st[1] + g * a.dk_st[2] + c] = (T)s;
+    else static_cast<T*>(a.dv)[b * a.dv_st[0] + key * a.dv_st[1] + g * a.dv_st[2] + c - a.d] = (T)s;
   }
 }
 
@@ -526,14 +592,23 @@ int launch_table(const Args& a, const float* partial, int64_t rows, hipStream_t 
 constexpr int rows_per_group(int M) { return M <= 64 ? 16 : 32; }
 
 struct Work {
-  size_t delta, far, partial, total;
-  int groups;
+  size_t delta, far, partial, shares, total;
+  int groups, parts;
 };
+
+// Query heads of a group in workgroups of their own: where the key tiles alone leave compute units idle, or a causal
+// problem, whose first keys are seen by all rows and whose last by few, would wait for its longest workgroup.
+int parts_of(const Args& a) {
+  if (a.rep == 1) return 1;
+  const int64_t tiles = (int64_t)a.B * a.G * ((a.N + 63) / 64);
+  return tiles < 2048 ? a.rep : 1;
+}
 Work work_of(const Args& a) {
   Work w;
   if (short_bwd_route(a)) {
     w.groups = short_slots(a);
-    w.delta = w.far = w.partial = 0;
+    w.delta = w.far = w.partial = w.shares = 0;
+    w.parts = 1;
     w.total = a.want_table ? align_up((size_t)w.groups * a.H * a.buckets * sizeof(float), 256) : 0;
     return w;
   }
@@ -541,7 +616,9 @@ Work work_of(const Args& a) {
   w.delta = 0;
   w.far = align_up((size_t)a.B * a.H * a.M * sizeof(float), 256);
   w.partial = w.far + (a.want_table ? align_up((size_t)a.B * a.H * w.groups * sizeof(float2), 256) : 0);
-  w.total = w.partial + (a.want_table ? align_up((size_t)a.B * a.H * w.groups * a.buckets * sizeof(float), 256) : 0);
+  w.shares = w.partial + (a.want_table ? align_up((size_t)a.B * a.H * w.groups * a.buckets * sizeof(float), 256) : 0);
+  w.parts = parts_of(a);
+  w.total = w.shares + (w.parts > 1 ? align_up((size_t)w.parts * a.B * a.N * a.G * 2 * a.d * sizeof(float), 256) : 0);
   return w;
 }
 
@@ -577,19 +654,29 @@ int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
 template <typename T, int DP>
 int launch_width(const Args& a, char* ws, const Work& w, hipStream_t stream) {
   using TL = Tile<T, DP>;
-  // 32 keys to a wave where its operands and sums fit the registers (fp32 at 128 wide: they do not)
-  constexpr int KB = sizeof(T) == 4 && DP >= 96 ? 1 : 2, BQ = 32;
+  // 32 keys to a wave where its operands and sums fit the registers (fp32 at 96 wide and more: they do not).  A narrow
+  // head leaves room for two waves per SIMD; a wide one gets workgroups of two waves: two of them share a compute unit,
+  // and twice as many of half the length even out the causal ones (decoder layer of 4096 positions, with a query head to a workgroup: 1350 -> 523 us).
+  constexpr int KB = sizeof(T) == 4 && DP >= 96 ? 1 : 2, BQ = 32, WAVES = DP <= (sizeof(T) == 4 ? 32 : 64) ? 4 : 2;
   const char* what = "hivt_relative_attn_bwd";
   const int rc = rows_per_group(a.M) == 16 ? launch_rows<T, DP, 1>(a, ws, w, stream) : launch_rows<T, DP, 2>(a, ws, w, stream);
   if (rc != HIVT_OK || a.N == 0) return rc;
-  const int64_t blocks = (int64_t)a.B * a.G * ((a.N + 64 * KB - 1) / (64 * KB));
+  Args b = a;
+  b.splits = w.parts;
+  b.partial = reinterpret_cast<float*>(ws + w.shares);
+  const int64_t blocks = (int64_t)a.B * a.G * w.parts * ((a.N + 16 * WAVES * KB - 1) / (16 * WAVES * KB));
   const size_t lds = (size_t)2 * BQ * TL::PITCH * sizeof(T) + BQ * sizeof(float4) + (size_t)bias_width(a) * sizeof(float);
   HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
   if (lds > 48 * 1024)
-    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&dkv_kernel<T, DP, KB, BQ>),
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&dkv_kernel<T, DP, KB, BQ, WAVES>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
-  hipLaunchKernelGGL((dkv_kernel<T, DP, KB, BQ>), dim3((unsigned)blocks), dim3(256), lds, stream, a);
+  hipLaunchKernelGGL((dkv_kernel<T, DP, KB, BQ, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), lds, stream, b);
   HIVT_CHECK_LAUNCH(what);
+  if (w.parts > 1) {
+    const int64_t pieces = ((int64_t)a.B * a.N * a.G * 2 * a.d + 255) / 256;
+    hipLaunchKernelGGL(group_kernel<T>, dim3((unsigned)(pieces < 65536 ? pieces : 65536)), dim3(256), 0, stream, b);
+    HIVT_CHECK_LAUNCH(what);
+  }
   return HIVT_OK;
 }
 

@@ -17,8 +17,9 @@ namespace {
 
 constexpr int kBN = 64;
 
+// Two waves to a SIMD, so that one's matrix instructions run beside the other's exponentials, where the registers allow.
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP >= 96 && QB == 2 ? 1 : 2) void fwd_kernel(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -90,8 +91,8 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
     if (t < t_end) {
       const int64_t k0 = (int64_t)t * kBN;
       auto keep = [&](int row) { return (bits >> row & 1) != 0; };
-      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, keep);
-      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, keep);
+      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, bits == ~0ull, keep);
+      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, bits == ~0ull, keep);
     }
   };
   seek();
@@ -106,18 +107,30 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
     __syncthreads();
     if (!active || (a.causal && k0 > pos_hi)) continue;
 
+    // A block's operands are read while the block before is multiplied (left alone, the compiler reads each right before
+    // its product, and two waves do not hide that).
     f32x4 s[4][QB];
+    Frag<T, TL::E> kf[2][TL::KSTEPS];
+#pragma unroll
+    for (int ks = 0; ks < TL::KSTEPS; ++ks) kf[0][ks] = TL::rows(kt, 0, ks, lane);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
+      if (kb < 3) {
+#pragma unroll
+        for (int ks = 0; ks < TL::KSTEPS; ++ks) kf[(kb + 1) & 1][ks] = TL::rows(kt, (kb + 1) * 16, ks, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) s[kb][qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int ks = 0; ks < TL::KSTEPS; ++ks) {
-        const Frag<T, TL::E> kf = TL::rows(kt, kb * 16, ks, lane);
+      for (int ks = 0; ks < TL::KSTEPS; ++ks)
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) Frag<T, TL::E>::mma(kf, qf[qb][ks], s[kb][qb]);
-      }
+        for (int qb = 0; qb < QB; ++qb) Frag<T, TL::E>::mma(kf[kb & 1][ks], qf[qb][ks], s[kb][qb]);
     }
+    constexpr int RING = sizeof(T) == 2 ? 4 : 2;
+    Frag<T, 8> vf[RING];  // and the first of the values' while the softmax runs
+#pragma unroll
+    for (int i = 0; i < RING && i < 2 * NB; ++i) vf[i] = TL::cols(vt, i / NB * 32, i % NB * 16, lane);
     // scores in base-2 exponent units, with the bias of their distance
     const int rel_hi = k0 + kBN - 1 - pos_lo, rel_lo = k0 - pos_hi;
     const bool far = rel_hi <= -a.sat || rel_lo >= hi;
@@ -125,28 +138,23 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const float* const tab = bias + slot[qb] * width;
-      if (far) {
-        const float c = tab[rel_hi <= -a.sat ? 0 : width - 1];
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[kb][qb][r] = fmaf(s[kb][qb][r], a.scale2, c);
-      } else {
+      // Far, whole tiles: one bias for all pairs, which waits until the exponent.  (A huge one may not: added to the score
+      // at once it takes the score's digits, and tiles have to agree on that.)  Other tiles put bias and mask into the
+      // scores; both then take the same way, so that no registers are moved between two.
+      float mul = a.scale2, add = tab[rel_hi <= -a.sat ? 0 : width - 1];
+      if (!__all(far && whole && a.scale2 > 0.0f && fabsf(add) <= kPlainBias)) {
+        mul = 1.0f;
+        add = 0.0f;
         const int rel0 = k0 + quad * 4 - pos[qb] + a.sat;
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            s[kb][qb][r] = fmaf(s[kb][qb][r], a.scale2, tab[min(max(rel0 + kb * 16 + r, 0), width - 1)]);
-      }
-      if (!whole) {
         const int lim = a.causal ? pos[qb] - k0 : kBN;  // keys of the tile up to here
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
           const uint32_t nibble = (uint32_t)(keys >> (kb * 16 + quad * 4));
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!(nibble >> r & 1) || kb * 16 + quad * 4 + r > lim) s[kb][qb][r] = -INFINITY;
+          for (int r = 0; r < 4; ++r) {
+            const float x = fmaf(s[kb][qb][r], a.scale2, tab[min(max(rel0 + kb * 16 + r, 0), width - 1)]);
+            s[kb][qb][r] = !(nibble >> r & 1) || kb * 16 + quad * 4 + r > lim ? -INFINITY : x;
+          }
         }
       }
       float top = s[0][qb][0];
@@ -154,14 +162,15 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[kb][qb][r]);
-      const float m_new = fmaxf(m[qb], quad_max(top));
+      const float m_new = fmaxf(m[qb], quad_max(fmaf(top, mul, add)));
       const float m_safe = m_new == -INFINITY ? 0.0f : m_new;  // a row without any allowed key so far
+      const float shift = add - m_safe;
       float sum = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          s[kb][qb][r] = fexp2(s[kb][qb][r] - m_safe);
+          s[kb][qb][r] = fexp2(fmaf(s[kb][qb][r], mul, shift));
           sum += s[kb][qb][r];
         }
       const float alpha = fexp2(m[qb] - m_safe);
@@ -182,9 +191,10 @@ __global__ __launch_bounds__(256) void fwd_kernel(const Args a) {
       for (int qb = 0; qb < QB; ++qb) pf[qb] = pair_frag<T>(s[2 * kk][qb], s[2 * kk + 1][qb]);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const Frag<T, 8> vf = TL::cols(vt, kk * 32, n * 16, lane);
+        const int at = kk * NB + n;
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) Frag<T, 8>::mma(vf, pf[qb], o[n][qb]);
+        for (int qb = 0; qb < QB; ++qb) Frag<T, 8>::mma(vf[at % RING], pf[qb], o[n][qb]);
+        if (at + RING < 2 * NB) vf[at % RING] = TL::cols(vt, (at + RING) / NB * 32, (at + RING) % NB * 16, lane);
       }
     }
   }

@@ -214,6 +214,12 @@ def test_long_axis_is_split_and_joined():
         check(q, k, v, table, o, False, 128)
 
 
+def test_many_sequences_with_shared_heads():
+    """Enough key tiles that a workgroup takes all heads of a group, instead of one with the shares added later."""
+    for causal in (False, True):
+        check(*inputs(520, 40, 70, 4, 2, 8, torch.float32, 8), causal=causal)
+
+
 def test_equal_calls_give_equal_bits():
     q, k, v, table, o = inputs(4, 200, 200, 8, 2, 32, torch.bfloat16, 32)
     first = check(q, k, v, table, o, True, 64)
