@@ -131,6 +131,8 @@ SIGNATURES = {
     "hivt_qk_norm_rotary_bwd": (c_int, [_P, _P, c_float, _P, c_size_t, _P]),
     "hivt_orthogonalize_workspace_bytes": (c_size_t, [_P, c_int32]),
     "hivt_orthogonalize": (c_int, [_P, c_int32, c_int32, c_int32, c_float, _P, c_size_t, _P]),
+    "hivt_muon_momentum": (c_int, [_P, _P, _P, _P, c_int32, _P, c_float, c_int32, _P]),
+    "hivt_muon_apply": (c_int, [_P, _P, _P, _P, c_int32, _P, _P, c_float, c_float, _P]),
     "hivt_set_matmul_bf16": (c_int, [c_int]),
     "hivt_spectral_norm_fwd": (c_int, [c_int32, _P, _P, _P, _P, _P, c_int32, c_float, _P, _P, _P, _P, _P]),
     "hivt_spectral_norm_bwd": (c_int, [c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P]),

@@ -1,0 +1,125 @@
+// The two elementwise halves of an optimiser step along orthogonalised momenta, over a list of matrices in few launches:
+//   momentum:  buf <- mu buf + g;  update = g + mu buf (Nesterov) or buf
+//   apply:     p <- p (1 - lr wd) - lr scale_i o
+// between which hivt_orthogonalize turns the updates into o.  Bound by memory (16 + 12 bytes an element); like the AdamW
+// update, tensors are cut into 4096-element pieces, a workgroup each, and a set found_inf leaves everything as it was.
+#include "common.h"
+
+namespace hivt {
+namespace {
+
+constexpr int kMuonTensors = 96;
+constexpr int kMuonPiece = 4096;
+
+struct MuonBatch {
+  float* a[kMuonTensors];        // momentum: buffer; apply: parameter
+  const float* b[kMuonTensors];  // momentum: gradient; apply: orthogonalised update
+  float* c[kMuonTensors];        // momentum: update
+  float scale[kMuonTensors];
+  int32_t n[kMuonTensors];
+  int32_t first[kMuonTensors];
+  int32_t count, nesterov;
+  const float* found_inf;
+  const float* lr_ptr;
+  float mu, lr, weight_decay;
+};
+
+template <bool APPLY>
+__global__ __launch_bounds__(256) void muon_kernel(const MuonBatch m) {
+  if (m.found_inf != nullptr && *m.found_inf == 1.0f) return;
+  int t = 0;
+  while (t + 1 < m.count && m.first[t + 1] <= (int)blockIdx.x) ++t;
+  const int begin = ((int)blockIdx.x - m.first[t]) * kMuonPiece, end = min(m.n[t], begin + kMuonPiece);
+  float* __restrict__ a = m.a[t];
+  const float* __restrict__ b = m.b[t];
+  float* __restrict__ c = m.c[t];
+  const float lr = APPLY && m.lr_ptr != nullptr ? *m.lr_ptr : m.lr;
+  const float keep = 1.0f - lr * m.weight_decay, rate = lr * m.scale[t], mu = m.mu;
+  auto one = [&](float& x, float y, float& z) {
+    if constexpr (APPLY) {
+      x = x * keep - rate * y;
+    } else {
+      x = mu * x + y;
+      z = m.nesterov ? y + mu * x : x;
+    }
+  };
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c);
+  if ((bits & 15) == 0 && (m.n[t] & 3) == 0) {
+    for (int i = begin + 4 * threadIdx.x; i < end; i += 4 * 256) {
+      float4 x = *reinterpret_cast<float4*>(a + i), z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 y = *reinterpret_cast<const float4*>(b + i);
+      one(x.x, y.x, z.x);
+      one(x.y, y.y, z.y);
+      one(x.z, y.z, z.z);
+      one(x.w, y.w, z.w);
+      *reinterpret_cast<float4*>(a + i) = x;
+      if constexpr (!APPLY) *reinterpret_cast<float4*>(c + i) = z;
+    }
+    return;
+  }
+  for (int i = begin + threadIdx.x; i < end; i += 256) {
+    float x = a[i], z = 0.0f;
+    one(x, b[i], z);
+    a[i] = x;
+    if constexpr (!APPLY) c[i] = z;
+  }
+}
+
+template <bool APPLY>
+int run(const char* what, const uint64_t* a, const uint64_t* b, const uint64_t* c, const float* scale, const int64_t* numels,
+        int32_t count, MuonBatch& m, hipStream_t stream) {
+  HIVT_REQUIRE(count >= 0, HIVT_ERR_ARG, "%s: negative tensor count", what);
+  if (count == 0) return HIVT_OK;
+  HIVT_REQUIRE(a && b && (APPLY ? scale != nullptr : c != nullptr) && numels, HIVT_ERR_ARG, "%s: null pointer", what);
+  for (int32_t i = 0; i < count; ++i) {
+    HIVT_REQUIRE(numels[i] >= 0 && numels[i] < ((int64_t)1 << 31) - kMuonPiece, HIVT_ERR_ARG, "%s: tensor %d has %lld elements",
+                 what, (int)i, (long long)numels[i]);
+    HIVT_REQUIRE(numels[i] == 0 || (a[i] && b[i] && (APPLY || c[i])), HIVT_ERR_ARG, "%s: tensor %d has a null pointer", what,
+                 (int)i);
+  }
+  for (int32_t i = 0; i < count;) {
+    int k = 0, pieces = 0;
+    for (; i < count && k < kMuonTensors; ++i) {
+      if (numels[i] == 0) continue;
+      m.a[k] = reinterpret_cast<float*>(a[i]);
+      m.b[k] = reinterpret_cast<const float*>(b[i]);
+      m.c[k] = APPLY ? nullptr : reinterpret_cast<float*>(c[i]);
+      m.scale[k] = APPLY ? scale[i] : 1.0f;
+      m.n[k] = (int32_t)numels[i];
+      m.first[k] = pieces;
+      pieces += (int)((numels[i] + kMuonPiece - 1) / kMuonPiece);
+      ++k;
+    }
+    if (k == 0) break;
+    m.count = k;
+    hipLaunchKernelGGL(muon_kernel<APPLY>, dim3((unsigned)pieces), dim3(256), 0, stream, m);
+    HIVT_CHECK_LAUNCH(what);
+  }
+  return HIVT_OK;
+}
+
+}  // namespace
+}  // namespace hivt
+
+using namespace hivt;
+
+extern "C" int hivt_muon_momentum(const uint64_t* buffers, const uint64_t* grads, const uint64_t* updates,
+                                  const int64_t* numels, int32_t count, const float* found_inf, float momentum,
+                                  int32_t nesterov, hivt_stream_t stream) {
+  MuonBatch m = {};
+  m.found_inf = found_inf;
+  m.mu = momentum;
+  m.nesterov = nesterov;
+  return run<false>("hivt_muon_momentum", buffers, grads, updates, nullptr, numels, count, m, (hipStream_t)stream);
+}
+
+extern "C" int hivt_muon_apply(const uint64_t* params, const uint64_t* directions, const float* scales, const int64_t* numels,
+                               int32_t count, const float* found_inf, const float* lr_ptr, float lr, float weight_decay,
+                               hivt_stream_t stream) {
+  MuonBatch m = {};
+  m.found_inf = found_inf;
+  m.lr_ptr = lr_ptr;
+  m.lr = lr;
+  m.weight_decay = weight_decay;
+  return run<true>("hivt_muon_apply", params, directions, nullptr, scales, numels, count, m, (hipStream_t)stream);
+}

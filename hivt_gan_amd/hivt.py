@@ -27,7 +27,7 @@ from .decoder import MLPDecoder
 from .global_interactor import GlobalInteractor
 from .local_encoder import LocalEncoder
 from .metrics import ValidationMetrics
-from .optim import FusedAdamW
+from .optim import FusedAdamW, Muon
 from .critics import multi_supported
 from .losses import (AdversarialDiscriminatorLoss, AdversarialGeneratorLoss, LaplaceNLLLoss,
                      SoftTargetCrossEntropyLoss, fused_supervised_losses, join_critic_streams)
@@ -61,11 +61,18 @@ class HiVT(nn.Module):
         # (train.py:76), where it reaches only that step: the GAN step optimises manually and is not clipped
         clip = kwargs.get("gradient_clip_val", 0.5)
         self.gradient_clip_val = float(clip) if clip else 0.0
+        # beyond the reference: "muon" steps the hidden matrices of the generator along orthogonalised momenta (optim.Muon,
+        # rate muon_lr) and the rest with AdamW; relative_positions: see TemporalEncoderLayer
+        self.optimizer = str(kwargs.get("optimizer", "adamw"))
+        if self.optimizer not in ("adamw", "muon"):
+            raise ValueError(f"optimizer must be 'adamw' or 'muon', got {self.optimizer!r}")
+        self.muon_lr = float(kwargs.get("muon_lr", 0.02))
 
         self.local_encoder = LocalEncoder(historical_steps=historical_steps, node_dim=node_dim, edge_dim=edge_dim,
                                           embed_dim=embed_dim, num_heads=num_heads, dropout=dropout,
                                           num_temporal_layers=num_temporal_layers, local_radius=local_radius,
-                                          parallel=parallel)
+                                          parallel=parallel,
+                                          relative_positions=bool(kwargs.get("relative_positions", False)))
         self.global_interactor = GlobalInteractor(historical_steps=historical_steps, embed_dim=embed_dim,
                                                   edge_dim=edge_dim, num_modes=num_modes, num_heads=num_heads,
                                                   num_layers=num_global_layers, dropout=dropout, rotate=rotate)
@@ -122,7 +129,8 @@ class HiVT(nn.Module):
 
     def configure_optimizers(self):
         """AdamW (all generator parameters decayed, ``models/hivt.py:428,444``) with cosine annealing;
-        a second AdamW without decay for the critics (``models/hivt.py:453``)."""
+        a second AdamW without decay for the critics (``models/hivt.py:453``).  With ``optimizer="muon"`` the generator's
+        hidden matrices take orthogonalised steps instead (``optim.Muon``; GPU parameters only)."""
         fused = next(self.parameters()).is_cuda
 
         def adamw(params, lr, weight_decay):
@@ -130,10 +138,20 @@ class HiVT(nn.Module):
                 return FusedAdamW(params, lr=lr, weight_decay=weight_decay)
             return torch.optim.AdamW(params, lr=lr, weight_decay=weight_decay)
 
+        def generator(params):
+            params = list(params)
+            if self.optimizer == "adamw":
+                return adamw(params, self.lr, self.weight_decay)
+            # the matrices between hidden features; first layers of two inputs and narrow heads stay with AdamW
+            matrices = [p for p in params if p.dim() == 2 and min(p.shape) >= 16]
+            chosen = {id(p) for p in matrices}
+            return Muon(matrices, [p for p in params if id(p) not in chosen], lr=self.muon_lr, weight_decay=self.weight_decay,
+                        adam_lr=self.lr, adam_weight_decay=self.weight_decay)
+
         if not self.use_gan:
-            opt = adamw(self.parameters(), self.lr, self.weight_decay)
+            opt = generator(self.parameters())
             return [opt], [torch.optim.lr_scheduler.CosineAnnealingLR(opt, T_max=self.T_max, eta_min=0.0)]
-        opt_g = adamw(self.generator_parameters(), self.lr, self.weight_decay)
+        opt_g = generator(self.generator_parameters())
         opt_d = adamw(self.critic_parameters(), self.critic_lr, 0.0)
         return [opt_g, opt_d], [torch.optim.lr_scheduler.CosineAnnealingLR(opt_g, T_max=self.T_max, eta_min=0.0)]
 

@@ -396,10 +396,25 @@ class ALEncoder(_EdgeAttentionBase):
 # Temporal encoder (dense; stock attention kernels)
 # ----------------------------------------------------------------------------------------------
 class TemporalEncoderLayer(nn.Module):
-    """Pre-norm self-attention + feed-forward block (``models/local_encoder.py:244-280``)."""
+    """Pre-norm self-attention + feed-forward block (``models/local_encoder.py:244-280``).
 
-    def __init__(self, embed_dim: int, num_heads: int = 8, dropout: float = 0.1) -> None:
+    ``relative_positions`` (beyond the reference): queries and keys of every head are normalised and rotated by their step
+    (``ops.qk_norm_rotary``), and a learned bias for each bucket of step distances joins the scores
+    (``ops.relative_attention``), for histories of any length; heads of an even width up to 128.  The attention weights
+    have no dropout then (the other three dropouts stay).  Adds the parameters ``q_norm``, ``k_norm`` [head width] and
+    ``relative_bias`` [32, heads]."""
+
+    MAX_DISTANCE = 128
+
+    def __init__(self, embed_dim: int, num_heads: int = 8, dropout: float = 0.1, relative_positions: bool = False) -> None:
         super().__init__()
+        self.relative_positions = bool(relative_positions)
+        if self.relative_positions:
+            if embed_dim % num_heads or embed_dim // num_heads % 2 or embed_dim // num_heads > 128:
+                raise ValueError(f"relative positions need heads of an even width up to 128, got {embed_dim} over {num_heads}")
+            self.q_norm = nn.Parameter(torch.ones(embed_dim // num_heads))
+            self.k_norm = nn.Parameter(torch.ones(embed_dim // num_heads))
+            self.relative_bias = nn.Parameter(torch.zeros(32, num_heads))
         self.self_attn = nn.MultiheadAttention(embed_dim=embed_dim, num_heads=num_heads, dropout=dropout)
         self.linear1 = nn.Linear(embed_dim, embed_dim * 4)
         self.dropout = nn.Dropout(dropout)
@@ -414,6 +429,12 @@ class TemporalEncoderLayer(nn.Module):
         mha = self.self_attn
         S, N, D = x.shape
         H = mha.num_heads
+        if self.relative_positions:
+            o = self._relative_attention(x, S)
+            if x.is_cuda:
+                return ops.fused_linear(o, mha.out_proj.weight, mha.out_proj.bias, dropout_p=self.dropout1.p,
+                                        training=self.training, residual=residual)
+            return residual + self.dropout1(mha.out_proj(o))
         if x.is_cuda and ops.temporal_attention_supported(S, D, H):
             qkv = ops.fused_linear(x, mha.in_proj_weight, mha.in_proj_bias)
             o = ops.temporal_attention(qkv, H, mha.dropout, self.training)
@@ -428,6 +449,40 @@ class TemporalEncoderLayer(nn.Module):
         o = F.scaled_dot_product_attention(q, k, v, dropout_p=mha.dropout if self.training else 0.0, is_causal=True)
         o = o.permute(2, 0, 1, 3).reshape(S, N, D)
         return residual + self.dropout1(mha.out_proj(o))
+
+    def _relative_attention(self, x: torch.Tensor, queries: int) -> torch.Tensor:
+        """Attention of the last ``queries`` steps of x [S, N, D] over all steps up to theirs -> [queries, N, D]."""
+        mha = self.self_attn
+        S, N, D = x.shape
+        H = mha.num_heads
+        if x.is_cuda:
+            qkv = ops.fused_linear(x, mha.in_proj_weight, mha.in_proj_bias)
+        else:
+            qkv = F.linear(x, mha.in_proj_weight, mha.in_proj_bias)
+        q, k, v = qkv.view(S, N, 3, H, D // H).transpose(0, 1).unbind(2)  # [N, S, H, d]
+        if x.is_cuda:
+            q, k = ops.qk_norm_rotary(q, k, self.q_norm, self.k_norm)
+            o = ops.relative_attention(q[:, S - queries:], k, v, self.relative_bias, causal=True,
+                                       max_distance=self.MAX_DISTANCE)
+            return o.transpose(0, 1).reshape(queries, N, D)
+        # CPU tensors: the formulas in the framework's operators
+        half = D // H // 2
+        angle = torch.arange(S, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(half, dtype=torch.float64) / half)
+        cos, sin = (f(angle).to(x.dtype)[:, None] for f in (torch.cos, torch.sin))
+
+        def turned(t, weight):
+            t = t * (t.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * weight
+            a, b = t[..., :half], t[..., half:]
+            return torch.cat((a * cos - b * sin, a * sin + b * cos), dim=-1)
+
+        q, k = turned(q, self.q_norm)[:, S - queries:].transpose(1, 2), turned(k, self.k_norm).transpose(1, 2)
+        exact, borders = ops.relative_buckets(self.relative_bias.shape[0], self.MAX_DISTANCE, False)
+        rel = torch.arange(S)[None] - torch.arange(S - queries, S)[:, None]
+        dist = (-rel).clamp(min=0)
+        bucket = torch.where(dist < exact, dist, exact + torch.bucketize(dist, torch.tensor(borders), right=True))
+        scores = (q @ k.transpose(2, 3)) * (D // H) ** -0.5 + self.relative_bias[bucket].permute(2, 0, 1)
+        o = torch.softmax(scores.masked_fill(rel > 0, float("-inf")), dim=-1) @ v.transpose(1, 2)
+        return o.permute(2, 0, 1, 3).reshape(queries, N, D)
 
     def _ff(self, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor:
         # residual + dropout2(linear2(dropout(relu(linear1(x)))))
@@ -449,7 +504,7 @@ class TemporalEncoderLayer(nn.Module):
     def forward(self, src: torch.Tensor, src_mask: Optional[torch.Tensor] = None,
                 src_key_padding_mask: Optional[torch.Tensor] = None, is_causal: bool = True) -> torch.Tensor:
         S, _, D = src.shape
-        if src.is_cuda and src.dtype == torch.float32 and D <= 128 and src.numel() > 0 \
+        if src.is_cuda and src.dtype == torch.float32 and D <= 128 and src.numel() > 0 and not self.relative_positions \
                 and ops.temporal_attention_supported(S, D, self.self_attn.num_heads):
             x = ops.pre_norm_temporal_attention(src, self.norm1, self.self_attn, self.dropout1.p, self.training)
         else:
@@ -468,6 +523,14 @@ class TemporalEncoderLayer(nn.Module):
         H, hd = mha.num_heads, D // mha.num_heads
         w, b = mha.in_proj_weight, mha.in_proj_bias
         gpu = src.is_cuda
+        if self.relative_positions:
+            o = self._relative_attention(ops.layer_norm(src, self.norm1), 1)[0]
+            if gpu:
+                x = ops.fused_linear(o, mha.out_proj.weight, mha.out_proj.bias, dropout_p=self.dropout1.p,
+                                     training=self.training, residual=src[-1])
+            else:
+                x = src[-1] + self.dropout1(mha.out_proj(o))
+            return self._ff_residual(x)
 
         def lin(x, weight, bias, **kw):
             if gpu:
@@ -523,9 +586,11 @@ def _step_rowptr(n: int, steps: int, device: torch.device) -> torch.Tensor:
 class _EncoderStack(nn.Module):
     """``layers`` + final ``norm`` under the key names of ``nn.TransformerEncoder``."""
 
-    def __init__(self, embed_dim: int, num_heads: int, num_layers: int, dropout: float) -> None:
+    def __init__(self, embed_dim: int, num_heads: int, num_layers: int, dropout: float, relative_positions: bool = False
+                 ) -> None:
         super().__init__()
-        self.layers = nn.ModuleList([TemporalEncoderLayer(embed_dim, num_heads, dropout) for _ in range(num_layers)])
+        self.layers = nn.ModuleList([TemporalEncoderLayer(embed_dim, num_heads, dropout, relative_positions)
+                                     for _ in range(num_layers)])
         self.norm = nn.LayerNorm(embed_dim)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -541,12 +606,13 @@ class _EncoderStack(nn.Module):
 
 
 class TemporalEncoder(nn.Module):
-    """Causal transformer over the history with a trailing class token (``models/local_encoder.py:205-241``)."""
+    """Causal transformer over the history with a trailing class token (``models/local_encoder.py:205-241``).
+    ``relative_positions``: see ``TemporalEncoderLayer``; the learned embedding of each step is added as before."""
 
     def __init__(self, historical_steps: int, embed_dim: int, num_heads: int = 8, num_layers: int = 4,
-                 dropout: float = 0.1) -> None:
+                 dropout: float = 0.1, relative_positions: bool = False) -> None:
         super().__init__()
-        self.transformer_encoder = _EncoderStack(embed_dim, num_heads, num_layers, dropout)
+        self.transformer_encoder = _EncoderStack(embed_dim, num_heads, num_layers, dropout, relative_positions)
         self.padding_token = nn.Parameter(torch.empty(historical_steps, 1, embed_dim))
         self.cls_token = nn.Parameter(torch.empty(1, 1, embed_dim))
         self.pos_embed = nn.Parameter(torch.empty(historical_steps + 1, 1, embed_dim))
@@ -585,7 +651,7 @@ class LocalEncoder(nn.Module):
 
     def __init__(self, historical_steps: int, node_dim: int, edge_dim: int, embed_dim: int, num_heads: int = 8,
                  dropout: float = 0.1, num_temporal_layers: int = 4, local_radius: float = 50,
-                 parallel: bool = False) -> None:
+                 parallel: bool = False, relative_positions: bool = False) -> None:
         super().__init__()
         self.historical_steps = historical_steps
         self.parallel = parallel
@@ -594,7 +660,8 @@ class LocalEncoder(nn.Module):
         self.aa_encoder = AAEncoder(historical_steps=historical_steps, node_dim=node_dim, edge_dim=edge_dim,
                                     embed_dim=embed_dim, num_heads=num_heads, dropout=dropout, parallel=parallel)
         self.temporal_encoder = TemporalEncoder(historical_steps=historical_steps, embed_dim=embed_dim,
-                                                num_heads=num_heads, dropout=dropout, num_layers=num_temporal_layers)
+                                                num_heads=num_heads, dropout=dropout, num_layers=num_temporal_layers,
+                                                relative_positions=relative_positions)
         self.al_encoder = ALEncoder(node_dim=node_dim, edge_dim=edge_dim, embed_dim=embed_dim, num_heads=num_heads,
                                     dropout=dropout)
 

@@ -12,6 +12,7 @@ framework's to rounding); ``use_library_kernel = False`` keeps the framework's k
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -219,3 +220,108 @@ class FusedAdamW(torch.optim.AdamW):
         out = super().step(closure)
         self._cache()
         return out
+
+
+class Muon(FusedAdamW):
+    """Steps along orthogonalised momenta for matrices, AdamW for everything else, as one optimizer.
+
+    ``matrices``: 2-D float32 GPU parameters (one list).  Their update is the momentum (``momentum``, Nesterov by default)
+    brought to singular values near 1 (``ops.orthogonalize``, ``steps`` steps) and scaled by sqrt(max(1, rows / cols)):
+    ``p <- p (1 - lr wd) - lr scale o``.  ``others``: any parameters, stepped as ``FusedAdamW`` does with ``adam_lr``,
+    ``betas``, ``adam_eps``.  The groups are ``param_groups[:-1]`` (AdamW, absent without ``others``) and
+    ``param_groups[-1]`` (``orthogonal=True``); schedulers, ``found_inf`` and recorded steps work as with ``FusedAdamW``."""
+
+    def __init__(self, matrices, others=(), lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7,
+                 adam_lr=1e-3, betas=(0.9, 0.999), adam_eps=1e-8, adam_weight_decay=0.0) -> None:
+        matrices, others = list(matrices), list(others)
+        if not matrices:
+            raise ValueError("no matrices: use FusedAdamW")
+        for p in matrices:
+            if p.dim() != 2 or p.dtype != torch.float32 or not p.is_cuda:
+                raise ValueError(f"orthogonalised steps are for 2-D float32 GPU parameters, got {p.dtype} {tuple(p.shape)} "
+                                 f"on {p.device}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum {momentum} must be in [0, 1)")
+        if not 1 <= int(steps) <= 16 or not eps > 0.0:
+            raise ValueError(f"steps {steps} must be 1 to 16 and eps {eps} positive")
+        groups = [dict(params=others, lr=adam_lr, weight_decay=adam_weight_decay)] if others else []
+        groups.append(dict(params=matrices, lr=lr, weight_decay=weight_decay, orthogonal=True, momentum=momentum,
+                           nesterov=bool(nesterov), steps=int(steps), ortho_eps=float(eps)))
+        super().__init__(groups, lr=adam_lr, betas=betas, eps=adam_eps, weight_decay=adam_weight_decay)
+
+    def __setstate__(self, state) -> None:
+        # (the framework's Adam expects a step counter in every state; momenta have none)
+        held = [st for st in state["state"].values() if "momentum_buffer" in st]
+        for st in held:
+            st["step"] = torch.zeros(())
+        super().__setstate__(state)
+        for st in held:
+            del st["step"]
+
+    def add_param_group(self, param_group) -> None:
+        if any(g.get("orthogonal") for g in self.param_groups):
+            raise ValueError("the group of matrices is the last one; hand all parameters to the constructor")
+        super().add_param_group(param_group)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if getattr(self, "grad_scale", None) is not None:
+            raise RuntimeError("Muon takes unscaled gradients")
+        groups = self.param_groups
+        on_library = True
+        if len(groups) > 1:
+            self.param_groups = groups[:-1]
+            try:
+                super().step()
+            finally:
+                self.param_groups = groups
+            on_library = self.last_step_on_library
+        self._matrix_step(groups[-1], len(groups) - 1)
+        self.last_step_on_library = on_library and isinstance(groups[-1]["lr"], float)
+        return loss
+
+    def _matrix_step(self, group, index: int) -> None:
+        from . import ops
+        from .ops_orthogonal import _outputs
+        from ._opsbase import _on_device
+        found_inf = getattr(self, "found_inf", None)
+        if found_inf is not None and (found_inf.dtype != torch.float32 or not found_inf.is_cuda):
+            raise TypeError("found_inf must be a float32 GPU scalar")
+        params, grads, buffers = [], [], []
+        for p in group["params"]:
+            if p.grad is None:
+                continue
+            if p.grad.is_sparse or p.grad.dtype != torch.float32 or not p.is_contiguous():
+                raise RuntimeError("orthogonalised steps take dense float32 gradients of contiguous parameters")
+            st = self.state[p]
+            if "momentum_buffer" not in st:
+                st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            params.append(p)
+            grads.append(p.grad.contiguous())
+            buffers.append(st["momentum_buffer"])
+        if not params:
+            return
+        device, count = params[0].device, len(params)
+        if any(p.device != device for p in params):
+            raise ValueError("the matrices of one optimizer must be on one device")
+        array = ctypes.c_uint64 * count
+        numels = (ctypes.c_int64 * count)(*[p.numel() for p in params])
+        scales = (ctypes.c_float * count)(*[math.sqrt(max(1.0, p.shape[0] / max(1, p.shape[1]))) for p in params])
+        updates = _outputs(params)
+        bad = found_inf.data_ptr() if found_inf is not None else None
+        with _on_device(params[0]):
+            stream = torch.cuda.current_stream(device).cuda_stream
+            _lib.call("hivt_muon_momentum", array(*map(_DATA_PTR, buffers)), array(*map(_DATA_PTR, grads)),
+                      array(*map(_DATA_PTR, updates)), numels, count, bad, float(group["momentum"]), int(group["nesterov"]),
+                      stream)
+            ops.orthogonalize(updates, steps=group["steps"], eps=group["ortho_eps"], out=updates)
+            lr = group["lr"]
+            lr_ptr = self._lr_scalar(index, group, device).data_ptr() if isinstance(lr, float) else None
+            if not torch.cuda.is_current_stream_capturing():
+                self.sync_lr()
+            _lib.call("hivt_muon_apply", array(*map(_DATA_PTR, params)), array(*map(_DATA_PTR, updates)), scales, numels, count,
+                      bad, lr_ptr, float(lr), float(group["weight_decay"]), stream)

@@ -621,6 +621,16 @@ size_t hivt_orthogonalize_workspace_bytes(const hivt_matrix* list, int32_t count
 int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_t dtype, int32_t steps, float eps, void* workspace,
                        size_t workspace_bytes, hivt_stream_t stream);
 
+/* The elementwise halves of an optimiser step along orthogonalised momenta (float tensors, host arrays of addresses):
+ *   momentum:  buffer <- momentum buffer + grad;  update = grad + momentum buffer (nesterov != 0) or buffer
+ *   apply:     param <- param (1 - lr weight_decay) - lr scale_i direction
+ * lr_ptr: optional device scalar that replaces lr; found_inf: optional device scalar, 1 leaves everything as it is. */
+int hivt_muon_momentum(const uint64_t* buffers, const uint64_t* grads, const uint64_t* updates, const int64_t* numels,
+                       int32_t count, const float* found_inf, float momentum, int32_t nesterov, hivt_stream_t stream);
+int hivt_muon_apply(const uint64_t* params, const uint64_t* directions, const float* scales, const int64_t* numels,
+                    int32_t count, const float* found_inf, const float* lr_ptr, float lr, float weight_decay,
+                    hivt_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------
  * Fused regression / classification loss (min over modes + Laplace NLL + soft-target CE)
  * ------------------------------------------------------------------------------------------ */
