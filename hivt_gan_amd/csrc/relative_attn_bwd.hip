@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2
   const int qtile = qtiles - 1 - inner;
   const int b = unit / a.H, h = unit % a.H, g = h / a.rep;
   const int width = bias_width(a), hi = bias_hi(a);
-  for (int e = tid; e < width; e += 256) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+  for (int e = tid; e < width; e += 256) bias[e] = bias2(a.table[(int64_t)entry_bucket(a, e) * a.H + h]);
 
   const int row0 = qtile * 64 * QB + wave * 16 * QB;
   const bool active = row0 < a.M;
@@ -143,19 +143,31 @@ __global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2
       for (int qb = 0; qb < QB; ++qb) {
         float mul = a.scale2, add = c;  // (see the forward)
         if (!plain) {
+          if (far) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, c);
+          } else {
+            const float* const at = bias + k0 + kk * 32 + quad * 4 - pos[qb] + a.sat + kMargin;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, at[i * 16 + r]);
+          }
           mul = 1.0f;
           add = 0.0f;
-          const int rel0 = k0 + kk * 32 + quad * 4 - pos[qb] + a.sat;
-          const int lim = a.causal ? pos[qb] - k0 : kBN;
+          if (!whole) {
+            const int lim = a.causal ? pos[qb] - k0 : kBN;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float x = fmaf(s[i][qb][r], a.scale2, bias[min(max(rel0 + i * 16 + r, 0), width - 1)]);
-              const bool out = !(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim;
-              s[i][qb][r] = out ? -INFINITY : x;
-              dp[i][qb][r] = out ? 0.0f : dp[i][qb][r];
+              for (int r = 0; r < 4; ++r) {
+                const bool out = !(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim;
+                s[i][qb][r] = out ? -INFINITY : s[i][qb][r];
+                dp[i][qb][r] = out ? 0.0f : dp[i][qb][r];
+              }
             }
           }
         }
@@ -272,7 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(con
   for (int hr = 0; hr < heads; ++hr) {
     const int h = g * a.rep + part * heads + hr;
     __syncthreads();  // the head before has been finished by every wave
-    for (int e = tid; e < width; e += 64 * WAVES) bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
+    for (int e = tid; e < width; e += 64 * WAVES) bias[e] = bias2(a.table[(int64_t)entry_bucket(a, e) * a.H + h]);
     const T* const qbase = static_cast<const T*>(a.q) + b * a.q_st[0] + h * a.q_st[2];
     const T* const obase = static_cast<const T*>(a.d_out) + b * a.do_st[0] + h * a.do_st[2];
     const int64_t rowbase = ((int64_t)b * a.H + h) * a.M;
@@ -339,7 +351,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(con
                 ds[i][kb][r] = w * (ds[i][kb][r] - rs.z);
               }
             }
-        } else {
+        } else {  // (one loop, clamped: bias and mask in loops of their own, as in the other kernels, took a quarter more)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -349,7 +361,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(con
 #pragma unroll
               for (int kb = 0; kb < KB; ++kb) {
                 const int rel = key[kb] - pos0 - row;
-                const float add = bias[min(max(rel + a.sat, 0), width - 1)];
+                const float add = bias[min(max(rel + a.sat + kMargin, 0), width - 1)];
                 float w = fexp2(fmaf(p[i][kb][r], a.scale2, add) - rs.x) * rs.y;
                 float dp = ds[i][kb][r];
                 if (!keep[kb] || s0 + row >= a.M || (a.causal && rel > 0)) w = dp = 0.0f;
@@ -424,22 +436,22 @@ template <typename T, int DP, int QB>
 __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __restrict__ far_sums,
                                                   float* __restrict__ partial) {
   using TL = Tile<T, DP>;
-  constexpr int ROWS = 16 * QB, PITCH = kBN + 4;
+  // sixteen rows at a time, each between margins of zeros, so that every diagonal has sixteen elements
+  constexpr int ROWS = 16 * QB, LEFT = 16, PITCH = LEFT + kBN + 16 + 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const skew = reinterpret_cast<float*>(smem);
-  float* const bias = skew + ROWS * PITCH;
-  const int width = bias_width(a), hi = bias_hi(a);
-  float* const diag = bias + width;
+  float* const bias = skew + 16 * PITCH;
+  const int hi = bias_hi(a);
+  float* const diag = bias + bias_width(a);
 
   const int lane = threadIdx.x, quad = lane >> 4;
   const int groups = (a.M + ROWS - 1) / ROWS;
   int unit, group;
   walk(blockIdx.x, a.B * a.H, groups, unit, group);
   const int b = unit / a.H, h = unit % a.H, g = h / a.rep;
-  for (int e = lane; e < width; e += 64) {
-    bias[e] = bias2(a.table[(int64_t)rel_bucket(a, e - a.sat) * a.H + h]);
-    diag[e] = 0.0f;
-  }
+  for (int e = lane; e < bias_width(a); e += 64) bias[e] = bias2(a.table[(int64_t)entry_bucket(a, e) * a.H + h]);
+  for (int e = lane; e < core_width(a); e += 64) diag[e] = 0.0f;
+  for (int e = lane; e < 16 * PITCH; e += 64) skew[e] = 0.0f;
   __syncthreads();
   const int row0 = group * ROWS;
   int pos[QB];
@@ -478,6 +490,7 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
     if (rel_hi <= -a.sat || rel_lo >= hi) continue;
     const uint64_t keys = tile_keys(a, b, k0, lane);
     if (keys == 0) continue;
+    f32x4 ds[4][QB];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       const int key = k0 + kb * 16 + (lane & 15);
@@ -501,35 +514,37 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const int rel0 = k0 + kb * 16 + quad * 4 - pos[qb];
-        f32x4 ds;
+        const float* const at = bias + rel0 + a.sat + kMargin;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float add = bias[min(max(rel0 + r + a.sat, 0), width - 1)];
-          const float p = fexp2(fmaf(s[qb][r], a.scale2, add) - m[qb]) * il[qb];
+          const float p = fexp2(fmaf(s[qb][r], a.scale2, at[r]) - m[qb]) * il[qb];
           const bool out = !(nibble >> r & 1) || (a.causal && rel0 + r > 0) || pos[qb] > pos_hi;
-          ds[r] = out ? 0.0f : p * (dp[qb][r] - delta[qb]);
+          ds[kb][qb][r] = out ? 0.0f : p * (dp[qb][r] - delta[qb]);
         }
-        *reinterpret_cast<f32x4*>(skew + (qb * 16 + (lane & 15)) * PITCH + kb * 16 + quad * 4) = ds;
       }
     }
-    __syncthreads();
-    // diagonal c: key - row = c - (ROWS - 1) within the tile
 #pragma unroll
-    for (int c0 = 0; c0 < kBN + ROWS - 1; c0 += 64) {
-      const int c = c0 + lane;
-      const int rel = k0 - pos_lo + c - (ROWS - 1);
-      float sum = 0.0f;
-#pragma unroll 8
-      for (int r = 0; r < ROWS; ++r) {
-        const int j = c - (ROWS - 1) + r;
-        if (j >= 0 && j < kBN) sum += skew[r * PITCH + j];
-      }
-      if (c < kBN + ROWS - 1) {
-        if (rel <= -a.sat) acc_l += sum;
-        else if (rel >= hi) acc_r += sum;
-        else diag[rel + a.sat] += sum;
-      }
+    for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+        *reinterpret_cast<f32x4*>(skew + (lane & 15) * PITCH + LEFT + kb * 16 + quad * 4) = ds[kb][qb];
       __syncthreads();
+      // diagonal c: key - row = c - 15 within the sixteen rows
+#pragma unroll
+      for (int c0 = 0; c0 < kBN + 15; c0 += 64) {
+        const int c = c0 + lane;
+        const int rel = k0 - (pos_lo + qb * 16) + c - 15;
+        const float* const from = skew + LEFT - 15 + min(c, kBN + 15);
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += from[r * (PITCH + 1)];
+        if (c < kBN + 15) {
+          if (rel <= -a.sat) acc_l += sum;
+          else if (rel >= hi) acc_r += sum;
+          else diag[rel + a.sat] += sum;
+        }
+        __syncthreads();
+      }
     }
   }
   const float2 fs = far_sums[(int64_t)unit * groups + group];
@@ -537,7 +552,7 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
   acc_r = wave_sum(acc_r) + fs.y;
   if (lane == 0) {
     diag[0] += acc_l;
-    diag[width - 1] += acc_r;
+    diag[core_width(a) - 1] += acc_r;
   }
   __syncthreads();
   const int side = a.bidirectional ? a.buckets / 2 : a.buckets;
@@ -638,7 +653,7 @@ int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
   hipLaunchKernelGGL((dq_kernel<T, DP, QB>), dim3((unsigned)blocks), dim3(256), lds, stream, a, far_sums);
   HIVT_CHECK_LAUNCH(what);
   if (a.want_table) {
-    const size_t lb = (size_t)16 * QB * (kBN + 4) * sizeof(float) + 2 * table;
+    const size_t lb = (size_t)16 * (kBN + 36) * sizeof(float) + table + (size_t)core_width(a) * sizeof(float);
     float* const partial = reinterpret_cast<float*>(ws + w.partial);
     if (lb > 48 * 1024)
       HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&bias_kernel<T, DP, QB>),

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP >= 96 && QB == 2 ? 1 : 2)
 
   const int width = bias_width(a), hi = bias_hi(a);
   for (int e = tid; e < width; e += 256) {
-    const int bucket = rel_bucket(a, e - a.sat);
+    const int bucket = entry_bucket(a, e);
     for (int s = 0; s < group; ++s) bias[s * width + e] = bias2(a.table[(int64_t)bucket * a.H + h0 + s]);
   }
 
@@ -143,17 +143,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP >= 96 && QB == 2 ? 1 : 2)
       // scores; both then take the same way, so that no registers are moved between two.
       float mul = a.scale2, add = tab[rel_hi <= -a.sat ? 0 : width - 1];
       if (!__all(far && whole && a.scale2 > 0.0f && fabsf(add) <= kPlainBias)) {
+        if (far) {
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[kb][qb][r] = fmaf(s[kb][qb][r], a.scale2, add);
+        } else {
+          const float* const at = tab + k0 + quad * 4 - pos[qb] + a.sat + kMargin;
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[kb][qb][r] = fmaf(s[kb][qb][r], a.scale2, at[kb * 16 + r]);
+        }
         mul = 1.0f;
         add = 0.0f;
-        const int rel0 = k0 + quad * 4 - pos[qb] + a.sat;
-        const int lim = a.causal ? pos[qb] - k0 : kBN;  // keys of the tile up to here
+        if (!whole) {
+          const int lim = a.causal ? pos[qb] - k0 : kBN;  // keys of the tile up to here
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-          const uint32_t nibble = (uint32_t)(keys >> (kb * 16 + quad * 4));
+          for (int kb = 0; kb < 4; ++kb) {
+            const uint32_t nibble = (uint32_t)(keys >> (kb * 16 + quad * 4));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = fmaf(s[kb][qb][r], a.scale2, tab[min(max(rel0 + kb * 16 + r, 0), width - 1)]);
-            s[kb][qb][r] = !(nibble >> r & 1) || kb * 16 + quad * 4 + r > lim ? -INFINITY : x;
+            for (int r = 0; r < 4; ++r)
+              s[kb][qb][r] = !(nibble >> r & 1) || kb * 16 + quad * 4 + r > lim ? -INFINITY : s[kb][qb][r];
           }
         }
       }

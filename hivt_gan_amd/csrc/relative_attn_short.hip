@@ -18,7 +18,8 @@ namespace rel {
 namespace {
 
 constexpr int64_t kMaxStride = 1 << 23;  // elements between positions: 64 of them stay within 2^31 bytes
-constexpr int kRel = 128;  // relative positions of at most 64 queries and 64 keys: 127
+// relative positions of at most 64 queries and 64 keys (127), with room for the rows behind the last query of a block
+constexpr int kFirst = 64, kRel = 192;
 
 // 32 rows of a tile in memory as reduction index, columns col0 + (lane & 15) as output index: see Tile::cols
 // (offsets within a sequence are 32-bit: see route)
@@ -38,11 +39,13 @@ __device__ __forceinline__ Frag<T, 8> cols_from(const T* base, int stride, int r
 
 __device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (1ull << n) - 1; }
 
-// The bias of every relative position -(M - 1) .. N - 1 (key index - query index), entry 0 first; base-2 exponent units.
+// The bias of every relative position -(M - 1) .. N - 1 (key index - query index) from entry kFirst on, in base-2 exponent
+// units, zero elsewhere.
 __device__ __forceinline__ void fill_bias(const Args& a, int h, float* bias, int lane) {
-  for (int e = lane; e < a.M + a.N - 1; e += 64) {
+  for (int i = lane; i < kRel; i += 64) {
+    const int e = i - kFirst;
     const int rel = min(max(e - (a.M - 1) - a.offset, -a.sat), bias_hi(a));
-    bias[e] = bias2(a.table[(int64_t)rel_bucket(a, rel) * a.H + h]);
+    bias[i] = e >= 0 && e < a.M + a.N - 1 ? bias2(a.table[(int64_t)rel_bucket(a, rel) * a.H + h]) : 0.0f;
   }
 }
 
@@ -57,6 +60,7 @@ __device__ __forceinline__ void weights(const Args& a, const Frag<T, Tile<T, DP>
   for (int qb = 0; qb < 2; ++qb) {
     const int q = q0 + qb * 16 + (lane & 15);
     const int lim = a.causal ? q + a.offset : a.N;
+    const float* const at = bias + kFirst + quad * 4 - q + a.M - 1;
     float top = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
@@ -67,8 +71,7 @@ __device__ __forceinline__ void weights(const Args& a, const Frag<T, Tile<T, DP>
       for (int r = 0; r < 4; ++r) {
         const int key = kb * 16 + quad * 4 + r;
         const bool ok = (keys >> key & 1) && key <= lim;
-        const int e = min(max(key - q + a.M - 1, 0), kRel - 1);  // (rows past the last query read some entry)
-        s[r] = ok ? fmaf(s[r], a.scale2, bias[e]) : -INFINITY;
+        s[r] = ok ? fmaf(s[r], a.scale2, at[kb * 16 + r]) : -INFINITY;
         top = fmaxf(top, s[r]);
       }
       p[kb][qb] = s;
@@ -291,6 +294,7 @@ __global__ __launch_bounds__(256, DP == 16 ? 3 : DP == 32 ? 2 : 1) void short_bw
       for (int kb = 0; kb < KB; ++kb) {
         const int key = kb * 16 + (lane & 15);
         const bool keep = (keys >> key & 1) != 0;
+        const float* const at = bias + kFirst + key - q0 - quad * 4 + a.M - 1;
         f32x4 pr[2], ds[2];
 #pragma unroll
         for (int qb = 0; qb < 2; ++qb) {
@@ -304,8 +308,7 @@ __global__ __launch_bounds__(256, DP == 16 ? 3 : DP == 32 ? 2 : 1) void short_bw
           for (int r = 0; r < 4; ++r) {
             const int q = q0 + qb * 16 + quad * 4 + r;
             const bool ok = keep && q < a.M && (!a.causal || key <= q + a.offset);
-            const int e = min(max(key - q + a.M - 1, 0), kRel - 1);
-            const float x = ok ? fexp2(fmaf(pr[qb][r], a.scale2, bias[e]) - mr[qb][r]) * ir[qb][r] : 0.0f;
+            const float x = ok ? fexp2(fmaf(pr[qb][r], a.scale2, at[-qb * 16 - r]) - mr[qb][r]) * ir[qb][r] : 0.0f;
             pr[qb][r] = x;
             ds[qb][r] = ok ? x * (ds[qb][r] - dr[qb][r]) : 0.0f;
           }

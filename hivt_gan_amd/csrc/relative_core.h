@@ -73,9 +73,16 @@ __device__ __forceinline__ int rel_bucket(const Args& a, int rel) {
   return rel > 0 ? a.buckets / 2 + side_bucket(a, rel) : side_bucket(a, -rel);
 }
 
-// entries of the LDS bias table of one head: relative positions -sat .. hi
+// The LDS bias table of one head: relative positions -sat .. hi, and kMargin more on either side that repeat the ends, so
+// that a tile that is not wholly beyond them (at most 64 keys and 32 rows, or the reverse) needs no clamping.
+constexpr int kMargin = 96;
 __host__ __device__ __forceinline__ int bias_hi(const Args& a) { return a.bidirectional ? a.sat : 0; }
-__host__ __device__ __forceinline__ int bias_width(const Args& a) { return a.sat + 1 + bias_hi(a); }
+__host__ __device__ __forceinline__ int core_width(const Args& a) { return a.sat + 1 + bias_hi(a); }
+__host__ __device__ __forceinline__ int bias_width(const Args& a) { return core_width(a) + 2 * kMargin; }
+// bucket of entry e of the table
+__device__ __forceinline__ int entry_bucket(const Args& a, int e) {
+  return rel_bucket(a, min(max(e - kMargin - a.sat, -a.sat), bias_hi(a)));
+}
 
 // bias in base-2 exponent units; the type's lowest value stays finite (a row of such biases is a row of equal ones)
 __device__ __forceinline__ float bias2(float b) {
