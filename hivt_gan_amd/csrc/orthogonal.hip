@@ -8,10 +8,12 @@
 // With X m x n that costs 3 m^2 n per phase and 5 m^3 or fewer per step (symmetric products at half, only the tiles on and
 // below the diagonal are computed) instead of 3 m^2 n + m^3 per step.  A phase forms G from the rounded X of the phase
 // before: what the squares of small singular values lose in G comes back only there.  Hence the phases' lengths: single
-// steps for nearly square matrices (n < 1.5 m), where that costs the same (20 m^3) and is the most accurate (a 64 x 64 one
-// with columns falling to 1e-3: 3e-7 off instead of 4e-6 with 2 + 3); else 1 + 2 + 2 for fp32 (47 instead of 65 m^3 at
-// n = 4 m) and 2 + 3 for 16-bit results (38 m^3; 128 x 20 of low rank: 3.0e-6 off, fp32 products by the definition 1.8e-6).
-// One phase of five would save more, but is 5e-3 off on matrices of low rank, even for 16-bit results too much.
+// steps for matrices that are not wide, where that costs little more or the same (20 m^3 for square ones) and is the most
+// accurate (a 64 x 64 one with columns falling to 1e-3: 3e-7 off instead of 4e-6 with 2 + 3); 1 + 2 + 2 for wide fp32 ones
+// (47 instead of 65 m^3 at n = 4 m), 2 + 3 for wide 16-bit ones (38 m^3; 128 x 20 of low rank: 3.0e-6 off, fp32 products by
+// the definition 1.8e-6).  Wide is n >= 2.5 m and n > 256 for fp32 (60 x 128: 2.2e-6 off in phases, by the definition
+// 1.2e-6), n >= 1.5 m for 16 bits.  One phase of five would save more, but is 5e-3 off on matrices of low rank, even for
+// 16-bit results too much.
 //
 // Bound by the matrix cores.  fp32 ones are eight times slower than 16-bit ones, so a value x is kept as two fp16 numbers
 // (hi = fp16(s x), lo = fp16(s x - hi)) and a product is hi hi + hi lo + lo hi with fp32 sums: 2^-24 of the value per
@@ -88,7 +90,11 @@ __device__ __forceinline__ int which(const Group& g, int block) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(lane < g.count && g.first[lane] <= block)) - 1);
 }
 
-__host__ __device__ inline bool is_wide(int64_t rows, int64_t cols) { return 2 * rows >= 3 * cols || 2 * cols >= 3 * rows; }
+// matrices whose steps are taken in phases (see above)
+__host__ __device__ inline bool is_wide(int64_t rows, int64_t cols, int dtype) {
+  const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return dtype == HIVT_F32 ? 2 * n >= 5 * m && n > 256 : 2 * n >= 3 * m;
+}
 
 __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
   if (dtype == HIVT_F32) return static_cast<const float*>(p)[i];
@@ -228,7 +234,7 @@ template <int BM_> struct Cfg {
   static constexpr int NPT = TILE * 2 / 16 / THREADS;               // 16-byte pieces of it per thread
 };
 
-template <int BM>
+template <int BM, bool SUMS>
 __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g, const Product p) {
   using C = Cfg<BM>;
   extern __shared__ __attribute__((aligned(16))) _Float16 lds_all[];  // [2][A, B][TILE]
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
   const int wi = (wave >> 1) * C::WM, wj = (wave & 1) * C::WN;
-  auto compute = [&](int buf) {
+  auto compute = [&](int buf, f32x16 (&acc)[C::TM][C::TN]) {
     const _Float16* const la = lds_all + buf * 2 * C::TILE;
     const _Float16* const lb = la + C::TILE;
 #pragma unroll
@@ -321,8 +327,28 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
 
   // one step: its products, then the next one's operands into the other buffer (whose readers passed the barrier of the
   // step before) and a later one's on their way.  The steps are an even number: sides are padded to 64.
+  // SUMS (fp32 in the smallest tile): each step has a sum of its own, as for the small matrices (200 x 1000: 2.4e-6 instead
+  // of 4.1e-6 off, by the definition 2.6e-6; 16 bits round coarser than either, and a bf16 1024 x 4096 takes 394 us without
+  // and 448 us with it)
   auto turn = [&](int buf, Step& r, int later) {
-    compute(buf);
+    if constexpr (SUMS) {
+      f32x16 part[C::TM][C::TN];
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) part[i][j][e] = 0.0f;
+      compute(buf, part);
+#pragma unroll
+      for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] += part[i][j][e];
+    } else {
+      compute(buf, acc);
+    }
     put(r, buf ^ 1);
     fetch(r, later);
     __syncthreads();
@@ -473,8 +499,12 @@ __global__ __launch_bounds__(Small<MP>::THREADS) void small_kernel(const Group g
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][e] = 0.0f;
   };
-  // 32 of the reduction index: A and B in blocks, `stride` blocks apart per 64 rows
+  // 32 of the reduction index: A and B in blocks, `stride` blocks apart per 64 rows.  Every step has a sum of its own, added
+  // to the whole in fp32: a matrix instruction cuts what it adds to a large sum short, and one chain over 512 is 3.3e-6 off
+  // in the result where this is 2.1e-6 (fp32 products by the definition: 1.9e-6).
   auto multiply = [&](f32x16 (&acc)[C::TN], const _Float16* A, int sa, const _Float16* B, int sb) {
+    f32x16 part[C::TN];
+    clear(part);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const int piece = ks * 2 + (lane >> 5);
@@ -491,11 +521,15 @@ __global__ __launch_bounds__(Small<MP>::THREADS) void small_kernel(const Group g
       }
 #pragma unroll
       for (int j = 0; j < C::TN; ++j) {
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[0][j], acc[j], 0, 0, 0);
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[1][j], acc[j], 0, 0, 0);
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1], fb[0][j], acc[j], 0, 0, 0);
+        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[0][j], part[j], 0, 0, 0);
+        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0], fb[1][j], part[j], 0, 0, 0);
+        part[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1], fb[0][j], part[j], 0, 0, 0);
       }
     }
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][e] += part[j][e];
   };
   constexpr int KB = MP / 32;  // steps of a square operand
   auto square = [&](const _Float16* A, const _Float16* B) {
@@ -579,7 +613,7 @@ __global__ __launch_bounds__(Small<MP>::THREADS) void small_kernel(const Group g
     fetch(r, Xt + ((int64_t)c * km + min(k, km - 1)) * 2 * kBlock, km, min(CB, nb - c));
   };
 
-  const int at_once = is_wide(mat.rows, mat.cols) ? 2 : 1;
+  const int at_once = is_wide(mat.rows, mat.cols, g.dtype) ? 2 : 1;
   int taken = 0;
   while (taken < steps_wanted) {
     const int steps = (steps_wanted - taken) % at_once != 0 ? 1 : at_once;
@@ -725,7 +759,7 @@ int64_t tiles_of(const Mat& a, int shape, int bm) {
   return shape == SHAPE_APPLY ? tm * tn : tm * (tm + 1) / 2;
 }
 
-template <int BM>
+template <int BM, bool SUMS = false>
 int launch_tiles(Group& g, const Product& p, hipStream_t stream) {
   using C = Cfg<BM>;
   const char* what = "hivt_orthogonalize";
@@ -737,9 +771,9 @@ int launch_tiles(Group& g, const Product& p, hipStream_t stream) {
   }
   const size_t lds = (size_t)4 * C::TILE * sizeof(_Float16);
   if (lds > 48 * 1024)
-    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<BM>),
+    HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<BM, SUMS>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
-  hipLaunchKernelGGL(product_kernel<BM>, dim3((unsigned)blocks), dim3(C::THREADS), lds, stream, g, p);
+  hipLaunchKernelGGL((product_kernel<BM, SUMS>), dim3((unsigned)blocks), dim3(C::THREADS), lds, stream, g, p);
   HIVT_CHECK_LAUNCH(what);
   return HIVT_OK;
 }
@@ -753,7 +787,7 @@ int launch_product(Group& g, const Product& p, hipStream_t stream) {
   }
   if (at256 >= 256) return launch_tiles<256>(g, p, stream);
   if (at128 >= 256) return launch_tiles<128>(g, p, stream);
-  return launch_tiles<64>(g, p, stream);
+  return g.dtype == HIVT_F32 ? launch_tiles<64, true>(g, p, stream) : launch_tiles<64>(g, p, stream);
 }
 
 // exponent of the scale of a product of k factors P (each at most 3.45)
@@ -911,7 +945,7 @@ extern "C" int hivt_orthogonalize(const hivt_matrix* list, int32_t count, int32_
       if (i < count) {
         const int64_t r = list[i].rows, c = list[i].cols;
         if (r * c == 0) continue;
-        if ((small_side(r, c) ? 2 : is_wide(r, c) ? 1 : 0) != kind) continue;
+        if ((small_side(r, c) ? 2 : is_wide(r, c, dtype) ? 1 : 0) != kind) continue;
         Mat& m = g.mats[g.count++];
         m.in = reinterpret_cast<const void*>(list[i].in);
         m.out = reinterpret_cast<void*>(list[i].out);
