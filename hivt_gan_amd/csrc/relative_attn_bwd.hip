@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2
   }
   const int pos_lo = min(row0, a.M - 1) + a.offset, pos_hi = max(min(row0 + 16 * QB, a.M) - 1, 0) + a.offset;
   const int wg_last = min((qtile + 1) * 64 * QB, a.M) - 1 + a.offset;
-  const int keys_end = a.causal ? min(a.N, wg_last + 1) : a.N;
+  const int keys_end = a.causal ? min(a.seen, wg_last + 1) : a.seen;
   const int t_end = keys_end > 0 ? (keys_end + kBN - 1) / kBN : 0;
 
   f32x4 dq[NB][QB];
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(con
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     key[kb] = key0 + kb * 16 + (lane & 15);
-    keep[kb] = key[kb] < a.N && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_sb + key[kb]] == 0);
+    keep[kb] = key[kb] < a.seen && (a.mask == nullptr || a.mask[(int64_t)b * a.mask_sb + key[kb]] == 0);
     any = any || keep[kb];
     const int64_t kc = min(key[kb], a.N - 1);
     const T* k = static_cast<const T*>(a.k) + b * a.k_st[0] + kc * a.k_st[1] + g * a.k_st[2];
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
     delta[qb] = live ? a.delta[at] : 0.0f;
   }
   const int pos_lo = row0 + a.offset, pos_hi = min(row0 + ROWS, a.M) - 1 + a.offset;
-  const int keys_end = a.causal ? min(a.N, pos_hi + 1) : a.N;
+  const int keys_end = a.causal ? min(a.seen, pos_hi + 1) : a.seen;
   // the tiles that are not far: rel_hi > -sat and rel_lo < hi
   const int t_begin = max(0, pos_lo - a.sat) / kBN;
   const int t_end = min(keys_end > 0 ? (keys_end + kBN - 1) / kBN : 0, max(0, (pos_hi + hi + kBN - 1) / kBN + 1));

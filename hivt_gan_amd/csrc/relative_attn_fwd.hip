@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP >= 96 && QB == 2 ? 1 : 2)
   const int pos_lo = first, pos_hi = max(last, 0) / group + a.offset;
   // the workgroup's range of tiles
   const int wg_last = (min((qtile + 1) * 64 * QB, rows) - 1) / group + a.offset;
-  const int keys_end = a.causal ? min(a.N, wg_last + 1) : a.N;
+  const int keys_end = a.causal ? min(a.seen, wg_last + 1) : a.seen;
   const int tiles = keys_end > 0 ? (keys_end + kBN - 1) / kBN : 0;
   const int t_begin = split * a.tiles_per_split, t_end = min(tiles, t_begin + a.tiles_per_split);
 
@@ -334,7 +334,7 @@ void plan(Args& a) {
   const int64_t rows = (int64_t)a.M * group;
   const int64_t qtiles = rows <= 64 ? 1 : (rows + 127) / 128;
   const int64_t work = (int64_t)a.B * (a.H / group) * qtiles;
-  const int tiles = (a.N + kBN - 1) / kBN;
+  const int tiles = (a.seen + kBN - 1) / kBN;
   // at least four tiles to a split: shorter ones spend their time on the start of a workgroup and on the join
   int64_t splits = work >= 512 ? 1 : 1024 / work;
   if (splits > tiles / 4) splits = tiles / 4;
@@ -460,6 +460,8 @@ int from_public(const char* what, const hivt_relative_attn* p, const int32_t* st
   a.rep = a.H / a.G;
   a.offset = (int32_t)p->q_offset;
   a.causal = p->causal != 0;
+  const int64_t reach = p->q_len + p->q_offset;  // (a cache's unwritten end may hold anything)
+  a.seen = !a.causal || reach >= p->k_len ? a.N : reach > 0 ? (int32_t)reach : 0;
   a.bidirectional = p->bidirectional != 0;
   a.buckets = (int32_t)p->buckets;
   a.exact = (int32_t)p->exact;

@@ -50,6 +50,7 @@ struct Args {
   int64_t mask_sb;
   int32_t B, M, N, H, G, d, rep;  // rep = H / G query heads to a key head
   int32_t offset;                 // position of query 0
+  int32_t seen;                   // keys that the last query may look at by position: those behind are not read
   int32_t causal, bidirectional;
   int32_t buckets, exact, nstarts, sat;
   int32_t pack;                   // rows of a tile run over (position, head of the group) instead of positions
@@ -296,10 +297,10 @@ __device__ __forceinline__ void store4(T* row, int col, int d, const f32x4& v) {
     if (col + j < d) row[col + j] = (T)v[j];
 }
 
-// Keys of a tile of 64 that may be looked at: bit j = key k0 + j exists and is not masked.  Uniform over the wave.
+// Keys of a tile of 64 that may be looked at: bit j = key k0 + j is seen by some position and not masked.  Uniform over the wave.
 __device__ __forceinline__ uint64_t tile_keys(const Args& a, int b, int k0, int lane) {
   const int key = k0 + lane;
-  bool ok = key < a.N;
+  bool ok = key < a.seen;
   if (ok && a.mask != nullptr) ok = a.mask[(int64_t)b * a.mask_sb + key] == 0;
   return __ballot(ok);
 }

@@ -35,6 +35,36 @@ def _outputs(matrices: Sequence[torch.Tensor]) -> List[torch.Tensor]:
     return out
 
 
+def _refuse_overlaps(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor]) -> None:
+    """An output may be its own matrix and nothing else: matrices of different sizes are worked on one after the other."""
+    spans = []
+    for i, (x, y) in enumerate(zip(ins, outs)):
+        if y.numel():
+            size = y.numel() * y.element_size()
+            spans.append((y.data_ptr(), y.data_ptr() + size, i, True))
+            if x.data_ptr() != y.data_ptr():
+                spans.append((x.data_ptr(), x.data_ptr() + size, i, False))
+    written = read = 0  # the furthest ends so far
+    for begin, end, i, is_out in sorted(spans):
+        if begin < written or (is_out and begin < read):
+            raise ValueError(f"output or matrix {i} shares memory with another output")
+        if is_out:
+            written = max(written, end)
+        else:
+            read = max(read, end)
+
+
+def _run(ins: Sequence[torch.Tensor], out: List[torch.Tensor], steps: int, eps: float) -> List[torch.Tensor]:
+    with _on_device(ins[0]):
+        ins = [x.contiguous() for x in ins]
+        array = matrix_list(ins, out)
+        need = _lib.value("hivt_orthogonalize_workspace_bytes", array, len(ins))
+        ws = _workspace(need, ins[0].device)
+        _lib.call("hivt_orthogonalize", array, len(ins), _DTYPES[ins[0].dtype], int(steps), float(eps), _p(ws), ws.numel(),
+                  _stream(ins[0]))
+    return out
+
+
 @torch.no_grad()
 def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float = 1e-7,
                   out: Optional[Sequence[torch.Tensor]] = None) -> List[torch.Tensor]:
@@ -42,8 +72,8 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float =
     ``steps`` times ``x <- a x + (b g + c g^2) x`` with g = x x^T (of the shorter side) and a, b, c = 3.4445, -4.7750,
     2.0315.  One type for the list, float32, bfloat16 or float16; any shapes up to 65536 a side.  The arithmetic is that of
     fp32 whatever the type, rounded once at the end; results are the same whatever else is in the list.  ``out``:
-    contiguous tensors to write to (the matrices themselves are allowed); without it, results of one shape are slices of one
-    allocation.  Not differentiable."""
+    contiguous tensors to write to (each may be its own matrix, and shares no memory with any other one or output); without
+    it, results of one shape are slices of one allocation.  Not differentiable."""
     matrices = list(matrices)
     if not matrices:
         return []
@@ -63,19 +93,14 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float =
         raise ValueError(f"eps must be positive, got {eps}")
     _need_gpu(*matrices)
     if out is None:
-        out = _outputs(matrices)
-    else:
-        out = list(out)
-        if len(out) != len(matrices):
-            raise ValueError(f"{len(matrices)} matrices, {len(out)} outputs")
-        for x, y in zip(matrices, out):
-            if y.shape != x.shape or y.dtype != dtype or y.device != device or not y.is_contiguous():
-                raise ValueError(f"an output must be contiguous {dtype} {tuple(x.shape)} on {device}")
-    with _on_device(matrices[0]):
-        ins = [x.contiguous() for x in matrices]
-        array = matrix_list(ins, out)
-        need = _lib.value("hivt_orthogonalize_workspace_bytes", array, len(ins))
-        ws = _workspace(need, device)
-        _lib.call("hivt_orthogonalize", array, len(ins), _DTYPES[dtype], int(steps), float(eps), _p(ws), ws.numel(),
-                  _stream(ins[0]))
-    return out
+        return _run(matrices, _outputs(matrices), steps, eps)
+    out = list(out)
+    if len(out) != len(matrices):
+        raise ValueError(f"{len(matrices)} matrices, {len(out)} outputs")
+    for x, y in zip(matrices, out):
+        if y.shape != x.shape or y.dtype != dtype or y.device != device or not y.is_contiguous():
+            raise ValueError(f"an output must be contiguous {dtype} {tuple(x.shape)} on {device}")
+    matrices = [x.contiguous() for x in matrices]
+    _refuse_overlaps(matrices, out)
+    torch.autograd.graph.increment_version([y for y in out if not y.is_inference()])
+    return _run(matrices, out, steps, eps)

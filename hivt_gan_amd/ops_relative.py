@@ -60,6 +60,11 @@ def _heads_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _recorded(*tensors: torch.Tensor) -> bool:
+    """Whether a call on them needs a node for its backward (one costs a single-token call half its time)."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
 def _tensor(t: Optional[torch.Tensor]):
     return (0, 0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
 
@@ -105,11 +110,9 @@ class _RelativeAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, mask, cfg, borders, scale):
-        want = any(ctx.needs_input_grad[:4])
-        out, stats = _forward(q, k, v, table, mask, cfg, borders, scale, want)
-        if want:
-            ctx.save_for_backward(q, k, v, table, mask, out, stats)
-            ctx.cfg = (cfg, borders, scale)
+        out, stats = _forward(q, k, v, table, mask, cfg, borders, scale, True)
+        ctx.save_for_backward(q, k, v, table, mask, out, stats)
+        ctx.cfg = (cfg, borders, scale)
         return out
 
     @staticmethod
@@ -121,26 +124,29 @@ class _RelativeAttention(torch.autograd.Function):
         return (*[g if need else None for g, need in zip(grads, ctx.needs_input_grad)], d_table, None, None, None, None)
 
 
+def _self_forward(qkv, table, heads, mask, cfg, borders, scale, want_stats):
+    s, n, three_d = qkv.shape
+    q, k, v = qkv.view(s, n, 3, heads, three_d // (3 * heads)).transpose(0, 1).unbind(2)
+    out = torch.empty(s, n, heads, q.shape[-1], dtype=qkv.dtype, device=qkv.device)
+    stats = torch.empty(n * heads, s, 2, dtype=torch.float32, device=qkv.device) if want_stats else None
+    with _on_device(qkv):
+        args = _block(cfg, q, k, v, table, mask, out.transpose(0, 1), stats)
+        need = _lib.value("hivt_relative_attn_fwd_workspace_bytes", args, borders)
+        ws = _workspace(need, qkv.device) if need else None
+        _lib.call("hivt_relative_attn_fwd", args, borders, scale, _p(ws), need, _stream(qkv))
+    return out, stats
+
+
 class _RelativeSelfAttention(torch.autograd.Function):
     """The same on the fused projection [S, N, 3 D]: the three gradients are written where the projection's products
     read them."""
 
     @staticmethod
     def forward(ctx, qkv, table, heads, mask, cfg, borders, scale):
-        s, n, three_d = qkv.shape
-        q, k, v = qkv.view(s, n, 3, heads, three_d // (3 * heads)).transpose(0, 1).unbind(2)
-        want = any(ctx.needs_input_grad[:2])
-        out = torch.empty(s, n, heads, q.shape[-1], dtype=qkv.dtype, device=qkv.device)
-        stats = torch.empty(n * heads, s, 2, dtype=torch.float32, device=qkv.device) if want else None
-        with _on_device(qkv):
-            args = _block(cfg, q, k, v, table, mask, out.transpose(0, 1), stats)
-            need = _lib.value("hivt_relative_attn_fwd_workspace_bytes", args, borders)
-            ws = _workspace(need, qkv.device) if need else None
-            _lib.call("hivt_relative_attn_fwd", args, borders, scale, _p(ws), need, _stream(qkv))
-        if want:
-            ctx.save_for_backward(qkv, table, mask, out, stats)
-            ctx.cfg = (heads, cfg, borders, scale)
-        return out.view(s, n, three_d // 3)
+        out, stats = _self_forward(qkv, table, heads, mask, cfg, borders, scale, True)
+        ctx.save_for_backward(qkv, table, mask, out, stats)
+        ctx.cfg = (heads, cfg, borders, scale)
+        return out.flatten(2)
 
     @staticmethod
     @once_differentiable
@@ -206,12 +212,15 @@ def relative_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table:
     ``table`` float32 [buckets, H] (see ``relative_buckets``; ``bidirectional`` defaults to ``not causal``).  Query i
     stands at position i + ``query_offset``, by default N - M, so that the queries are the last of the keys: with M = 1
     the call is one step of a sequence.  ``key_mask`` [B, N]: True leaves a key out, whatever it and its value hold; a
-    query without any key gives zeros and passes no gradient.  (The causal rule alone does not shield a row from a NaN or
-    an infinity in a later value: weights of zero are multiplied with it.)  Deterministic; scores, weights and sums are
+    query without any key gives zeros and passes no gradient.  With ``causal``, keys behind the last query are not read (the
+    unwritten end of a cache).  (Between the queries of one call the causal rule alone does not shield a row from a NaN or an
+    infinity in a later value: weights of zero are multiplied with it.)  Deterministic; scores, weights and sums are
     fp32, weights enter the product with v and score gradients the products with q and k in the tensors' type."""
     mask, cfg, borders, scale = _check(q, k, v, table, key_mask, causal, max_distance, bidirectional, scale, query_offset)
-    return _RelativeAttention.apply(_heads_last(q), _heads_last(k), _heads_last(v), table.contiguous(), mask, cfg, borders,
-                                    scale)
+    q, k, v, table = _heads_last(q), _heads_last(k), _heads_last(v), table.contiguous()
+    if _recorded(q, k, v, table):
+        return _RelativeAttention.apply(q, k, v, table, mask, cfg, borders, scale)
+    return _forward(q, k, v, table, mask, cfg, borders, scale, False)[0]
 
 
 def relative_self_attention(qkv: torch.Tensor, table: torch.Tensor, num_heads: int, causal: bool = True,
@@ -225,4 +234,7 @@ def relative_self_attention(qkv: torch.Tensor, table: torch.Tensor, num_heads: i
     s, n, three_d = qkv.shape
     q, k, v = qkv.view(s, n, 3, num_heads, three_d // (3 * num_heads)).transpose(0, 1).unbind(2)
     mask, cfg, borders, scale = _check(q, k, v, table, key_mask, causal, max_distance, bidirectional, None, None)
-    return _RelativeSelfAttention.apply(qkv, table.contiguous(), int(num_heads), mask, cfg, borders, scale)
+    table = table.contiguous()
+    if _recorded(qkv, table):
+        return _RelativeSelfAttention.apply(qkv, table, int(num_heads), mask, cfg, borders, scale)
+    return _self_forward(qkv, table, int(num_heads), mask, cfg, borders, scale, False)[0].flatten(2)

@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._opsbase import _need_gpu, _on_device, _p, _stream, _unsupported, _workspace
-from .ops_relative import _DTYPES, _heads_last, _tensor
+from .ops_relative import _DTYPES, _heads_last, _recorded, _tensor
 
 _Block = ctypes.c_int64 * 48  # hivt_qk_norm_rotary: 64-bit members only
 
@@ -36,15 +36,20 @@ def _block(q, k, wq, wk, positions, rotary_dim, interleaved, out=(None, None), d
                   0 if dw[1] is None else dw[1].data_ptr())
 
 
+def _forward(q, k, wq, wk, positions, rotary_dim, theta, interleaved, eps):
+    out = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    wq32, wk32 = wq.float().contiguous(), wk.float().contiguous()
+    with _on_device(q):
+        _lib.call("hivt_qk_norm_rotary_fwd", _block(q, k, wq32, wk32, positions, rotary_dim, interleaved, out),
+                  _rates(rotary_dim, theta), eps, _stream(q))
+    return out
+
+
 class _QKNormRotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, wq, wk, positions, rotary_dim, theta, interleaved, eps):
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
-        wq32, wk32 = wq.float().contiguous(), wk.float().contiguous()
-        with _on_device(q):
-            _lib.call("hivt_qk_norm_rotary_fwd", _block(q, k, wq32, wk32, positions, rotary_dim, interleaved, out),
-                      _rates(rotary_dim, theta), eps, _stream(q))
+        out = _forward(q, k, wq, wk, positions, rotary_dim, theta, interleaved, eps)
         ctx.save_for_backward(q, k, wq, wk, positions)
         ctx.cfg = (rotary_dim, theta, interleaved, eps)
         return out
@@ -106,5 +111,6 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     for t in (k, q_weight, k_weight, positions):
         if t is not None and t.device != q.device:
             raise ValueError(f"tensors on {q.device} and {t.device}")
-    return _QKNormRotary.apply(_heads_last(q), _heads_last(k), q_weight, k_weight, positions, rotary_dim, float(theta),
-                               int(bool(interleaved)), float(eps))
+    args = (_heads_last(q), _heads_last(k), q_weight, k_weight, positions, rotary_dim, float(theta), int(bool(interleaved)),
+            float(eps))
+    return _QKNormRotary.apply(*args) if _recorded(*args[:4]) else _forward(*args)

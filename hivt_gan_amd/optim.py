@@ -285,8 +285,7 @@ class Muon(FusedAdamW):
         return loss
 
     def _matrix_step(self, group, index: int) -> None:
-        from . import ops
-        from .ops_orthogonal import _outputs
+        from .ops_orthogonal import _outputs, _run
         from ._opsbase import _on_device
         found_inf = getattr(self, "found_inf", None)
         if found_inf is not None and (found_inf.dtype != torch.float32 or not found_inf.is_cuda):
@@ -318,10 +317,11 @@ class Muon(FusedAdamW):
             _lib.call("hivt_muon_momentum", array(*map(_DATA_PTR, buffers)), array(*map(_DATA_PTR, grads)),
                       array(*map(_DATA_PTR, updates)), numels, count, bad, float(group["momentum"]), int(group["nesterov"]),
                       stream)
-            ops.orthogonalize(updates, steps=group["steps"], eps=group["ortho_eps"], out=updates)
+            _run(updates, updates, group["steps"], group["ortho_eps"])
             lr = group["lr"]
             lr_ptr = self._lr_scalar(index, group, device).data_ptr() if isinstance(lr, float) else None
             if not torch.cuda.is_current_stream_capturing():
                 self.sync_lr()
             _lib.call("hivt_muon_apply", array(*map(_DATA_PTR, params)), array(*map(_DATA_PTR, updates)), scales, numels, count,
                       bad, lr_ptr, float(lr), float(group["weight_decay"]), stream)
+        torch.autograd.graph.increment_version(params)  # (a graph that still needs the old values says so)

@@ -564,7 +564,7 @@ typedef struct {
   int64_t key_mask, mask_stride; /* uint8 [batch][k_len], rows mask_stride apart; address 0: no mask */
   int64_t out, out_stride[3];
   int64_t stats;                 /* float2 [batch * heads][q_len], written by the forward (0: not wanted) */
-  /* backward only; dk, dv and d_table may be 0 together with nothing else */
+  /* backward only; all three gradients are written, also where they are zero */
   int64_t d_out, d_out_stride[3], dq, dq_stride[3], dk, dk_stride[3], dv, dv_stride[3];
   int64_t d_table;               /* float [buckets][heads]; 0: not wanted */
 } hivt_relative_attn;
@@ -609,7 +609,8 @@ int hivt_qk_norm_rotary_bwd(const hivt_qk_norm_rotary* p, const double* rates, f
  *
  *   X = in / (|in| + eps) (Frobenius norm), then `steps` times X <- a X + (b G + c G^2) X, G = X X' (X' X for a matrix
  *   with more rows than columns), with a, b, c = 3.4445, -4.7750, 2.0315: the singular values go near 1.  out = X.
- * in and out are contiguous row-major matrices of one type; in == out is allowed.  The host array is read before the
+ * in and out are contiguous row-major matrices of one type; in == out of
+ * one entry is allowed; an output shares memory with no other entry.  The host array is read before the
  * call returns.  Results are accurate to fp32 (see the kernels) and do not depend on what else is in the list.
  * ------------------------------------------------------------------------------------------ */
 typedef struct {

@@ -240,3 +240,14 @@ def test_operators_in_a_row():
     for direction, g in zip(ops.orthogonalize(list(grads[:3])), grads[:3]):
         want = orthogonal64(g.cpu().double())
         assert float((direction.cpu().double() - want).norm()) <= 3e-5 * float(want.norm())
+
+
+def test_a_graph_older_than_the_step_is_refused():
+    w = torch.randn(8, 8, device=DEV, requires_grad=True)
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    opt = Muon([w])
+    old = (x @ w).sum()
+    w.grad = torch.randn(8, 8, device=DEV)
+    opt.step()
+    with pytest.raises(RuntimeError, match="inplace"):
+        old.backward()

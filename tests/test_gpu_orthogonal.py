@@ -173,3 +173,16 @@ def test_refusals():
         ops.orthogonalize([torch.zeros(1, 65537, device=DEV)])
     with pytest.raises(RuntimeError, match="GPU only"):
         ops.orthogonalize([x.cpu()])
+
+
+def test_outputs_that_share_memory():
+    store = torch.randn(12, 70, device=DEV)
+    a, b, c = store[:4], store[4:8], store[8:]
+    want = ops.orthogonalize([a, b])
+    for ins, outs in (([a, b], [b, a]), ([a, b], [c, c]), ([a, b], [c, a]), ([a], [store[1:5]])):
+        with pytest.raises(ValueError, match="shares memory"):
+            ops.orthogonalize(ins, out=outs)
+    version = store._version
+    got = ops.orthogonalize([a, b], out=[a, c])
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a, want[0])
+    assert store._version > version

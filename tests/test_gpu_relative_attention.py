@@ -345,6 +345,34 @@ def test_offsets_beyond_32_bits():
     check(far, k, v, table, o, True)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,first", [(1, 40, 22), (3, 32, 10), (1, 700, 300), (19, 300, 100), (90, 300, 130), (70, 200, -30),
+                                       (5, 64, -5)])
+def test_unwritten_end_of_a_cache(dtype, M, N, first):
+    """Causal, behind the last query's position the keys and values are not numbers; nothing sees them."""
+    H, G, d = 4, 2, 24
+    q, k, v, table, o = inputs(2, M, N, H, G, d, dtype, 8)
+    written = max(0, M + first)
+    for clean in (k, v):
+        clean[:, written:] = 0.0
+    want, want_grads = check(q, k, v, table, o, True, offset=first)
+    k[:, written:], v[:, written:] = math.nan, math.inf
+    leaves = [t.requires_grad_(True) for t in (q, k, v, table)]
+    out = ops.relative_attention(*leaves, causal=True, max_distance=16, query_offset=first)
+    grads = torch.autograd.grad(out, leaves, o)
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(grads, want_grads))
+    assert not bool(grads[1][:, written:].any()) and not bool(grads[2][:, written:].any())
+
+
+def test_without_gradients_equal_bits():
+    q, k, v, table, o = inputs(2, 70, 90, 4, 2, 16, torch.bfloat16, 8)
+    want = ops.relative_attention(q, k, v, table.requires_grad_(True), causal=True, max_distance=16)
+    assert want.requires_grad
+    with torch.no_grad():
+        got = ops.relative_attention(q, k, v, table, causal=True, max_distance=16)
+    assert not got.requires_grad and torch.equal(got, want)
+
+
 def test_refusals():
     q, k, v, table, o = inputs(1, 8, 8, 4, 2, 16, torch.float32, 8)
     call = ops.relative_attention

@@ -52,3 +52,84 @@ def test_rotary_argument_block_matches_the_header():
             size = re.search(r"\[(\d+)\]", name)
             members += int(size.group(1)) if size else 1
     assert ctypes.sizeof(ops_rotary._Block) == 8 * members
+
+
+def _cpu(*shape, dtype=None):
+    import torch
+    return torch.zeros(*shape, dtype=dtype or torch.float32)
+
+
+def test_relative_attention_refuses_on_the_host():
+    import torch
+    from hivt_gan_amd import ops
+    q, k, table = _cpu(2, 5, 4, 16), _cpu(2, 7, 2, 16), _cpu(32, 4)
+    for args, kwargs, error in (
+            ((q.double(), k.double(), k.double(), table), {}, TypeError),
+            ((q, k.half(), k, table), {}, TypeError),
+            ((q[0], k, k, table), {}, ValueError),
+            ((q, k, k[:, :6], table), {}, ValueError),
+            ((q, k[:1], k[:1], table), {}, ValueError),
+            ((q, _cpu(2, 7, 3, 16), _cpu(2, 7, 3, 16), table), {}, ValueError),
+            ((q, k, k, table[:, :3]), {}, ValueError),
+            ((q, k, k, table.half()), {}, ValueError),
+            ((_cpu(2, 5, 4, 130), _cpu(2, 7, 2, 130), _cpu(2, 7, 2, 130), table), {}, ops.UnsupportedShapeError),
+            ((_cpu(2, 5, 4, 0), _cpu(2, 7, 2, 0), _cpu(2, 7, 2, 0), table), {}, ops.UnsupportedShapeError),
+            ((q, k, k, table), dict(key_mask=_cpu(2, 7)), ValueError),
+            ((q, k, k, table), dict(key_mask=_cpu(2, 6, dtype=torch.bool)), ValueError),
+            ((q, k, k, table), {}, RuntimeError)):  # on the CPU
+        with pytest.raises(error):
+            ops.relative_attention(*args, **kwargs)
+    with pytest.raises(ValueError):
+        ops.relative_self_attention(_cpu(5, 2, 50), table, 4)
+    with pytest.raises(ValueError):
+        ops.relative_self_attention(_cpu(5, 2, 48), table, 0)
+
+
+def test_norm_and_rotation_refuse_on_the_host():
+    import torch
+    from hivt_gan_amd import ops
+    q, k, w = _cpu(2, 5, 4, 16), _cpu(2, 5, 2, 16), _cpu(16)
+    for args, kwargs, error in (
+            ((q.double(), k.double(), w, w), {}, TypeError),
+            ((q, k.half(), w, w), {}, TypeError),
+            ((q, k[:, :4], w, w), {}, ValueError),
+            ((q[..., :15], k[..., :15], w[:15], w[:15]), {}, ops.UnsupportedShapeError),
+            ((_cpu(1, 1, 1, 258), _cpu(1, 1, 1, 258), _cpu(258), _cpu(258)), {}, ops.UnsupportedShapeError),
+            ((q, k, w[:8], w), {}, ValueError),
+            ((q, k, w.half(), w), {}, ValueError),
+            ((q, k, w, w), dict(rotary_dim=18), ValueError),
+            ((q, k, w, w), dict(rotary_dim=5), ValueError),
+            ((q, k, w, w), dict(theta=0.0), ValueError),
+            ((q, k, w, w), dict(theta=float("nan")), ValueError),
+            ((q, k, w, w), dict(eps=0.0), ValueError),
+            ((q, k, w, w), dict(positions=_cpu(5)), ValueError),
+            ((q, k, w, w), dict(positions=_cpu(4, dtype=torch.int64)), ValueError),
+            ((q, k, w, w), {}, RuntimeError)):
+        with pytest.raises(error):
+            ops.qk_norm_rotary(*args, **kwargs)
+
+
+def test_orthogonalize_refuses_on_the_host():
+    import torch
+    from hivt_gan_amd import ops, ops_orthogonal
+    x = _cpu(4, 6)
+    assert ops.orthogonalize([]) == []
+    for args, kwargs, error in (
+            (([x.double()],), {}, TypeError),
+            (([x, x.half()],), {}, TypeError),
+            (([x[0]],), {}, ValueError),
+            (([x],), dict(steps=0), ValueError),
+            (([x],), dict(steps=17), ValueError),
+            (([x],), dict(eps=0.0), ValueError),
+            (([x],), {}, RuntimeError)):
+        with pytest.raises(error):
+            ops.orthogonalize(*args, **kwargs)
+    # an output may be its own matrix, and no other's memory
+    store = _cpu(12, 6)
+    a, b, c = store[:4], store[4:8], store[8:]
+    for ins, outs in (([a, b], [a, b]), ([a, a], [b, c]), ([a], [b]), ([a, b], [c, b]), ([a, store[:0]], [a, store[:0]])):
+        ops_orthogonal._refuse_overlaps(ins, outs)
+    for ins, outs in (([a, b], [b, a]), ([a, b], [c, c]), ([a, b], [b, c]), ([a], [store[1:5]]), ([a, a], [a, c]),
+                      ([store[0:6], c], [store[0:6], store[5:9]]), ([store, a], [torch.empty_like(store), b])):
+        with pytest.raises(ValueError):
+            ops_orthogonal._refuse_overlaps(ins, outs)
