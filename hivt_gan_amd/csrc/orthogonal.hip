@@ -34,6 +34,7 @@
 namespace hivt {
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -96,12 +97,6 @@ __host__ __device__ inline bool is_wide(int64_t rows, int64_t cols, int dtype) {
   return dtype == HIVT_F32 ? 2 * n >= 5 * m && n > 256 : 2 * n >= 3 * m;
 }
 
-__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
-  if (dtype == HIVT_F32) return static_cast<const float*>(p)[i];
-  if (dtype == HIVT_BF16) return (float)static_cast<const __bf16*>(p)[i];
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-
 // sums of squares, in 64 bits: squares of small or large gradients leave the range of fp32
 __global__ __launch_bounds__(256) void sum_kernel(const Group g) {
   __shared__ double red[4];
@@ -110,11 +105,16 @@ __global__ __launch_bounds__(256) void sum_kernel(const Group g) {
   const int64_t total = (int64_t)a.rows * a.cols, from = (int64_t)(blockIdx.x - g.first[i]) * kSumChunk;
   const int left = (int)(total - from < kSumChunk ? total - from : kSumChunk);
   float v[kSumChunk / 256];  // all on their way at once
+  auto load = [&](auto* in) {
 #pragma unroll
-  for (int j = 0; j < kSumChunk / 256; ++j) {
-    const int at = threadIdx.x + j * 256;
-    v[j] = at < left ? load_as_float(a.in, from + at, g.dtype) : 0.0f;
-  }
+    for (int j = 0; j < kSumChunk / 256; ++j) {
+      const int at = threadIdx.x + j * 256;
+      v[j] = at < left ? (float)in[from + at] : 0.0f;
+    }
+  };
+  if (g.dtype == HIVT_F32) load(static_cast<const float*>(a.in));
+  else if (g.dtype == HIVT_BF16) load(static_cast<const __bf16*>(a.in));
+  else load(static_cast<const _Float16*>(a.in));
   double s = 0.0;
 #pragma unroll
   for (int j = 0; j < kSumChunk / 256; ++j) s += (double)v[j] * v[j];
@@ -174,12 +174,21 @@ __global__ __launch_bounds__(256) void convert_kernel(const Group g) {
   const bool flip = a.rows > a.cols;
   const int tc = l.np / 64, i0 = block / tc * 64, j0 = block % tc * 64;  // of the small x large form
   // read along the rows of the matrix as it lies
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    const int row = (flip ? j0 : i0) + r, col = (flip ? i0 : j0) + c;
-    const float v = row < a.rows && col < a.cols
-                        ? (float)(load_as_float(a.in, (int64_t)row * a.cols + col, g.dtype) * factor) : 0.0f;
-    tile[flip ? c : r][flip ? r : c] = v;
+  float in[16];
+  auto load = [&](auto* from) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int row = (flip ? j0 : i0) + j * 4 + (threadIdx.x >> 6), col = (flip ? i0 : j0) + (threadIdx.x & 63);
+      in[j] = row < a.rows && col < a.cols ? (float)from[(int64_t)row * a.cols + col] : 0.0f;
+    }
+  };
+  if (g.dtype == HIVT_F32) load(static_cast<const float*>(a.in));
+  else if (g.dtype == HIVT_BF16) load(static_cast<const __bf16*>(a.in));
+  else load(static_cast<const _Float16*>(a.in));
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int r = j * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
+    tile[flip ? c : r][flip ? r : c] = (float)(in[j] * factor);
   }
   __syncthreads();
   _Float16* const x = reinterpret_cast<_Float16*>(ws + l.x);
@@ -223,27 +232,34 @@ struct Product {
 // A workgroup's square of results.  Its loop is bound by latency if nothing is done about it: a step of 32 takes 200 to
 // 800 clocks of matrix work and its operands, just written by another kernel, over 2000 to arrive.  So AHEAD steps are on
 // their way into registers (variables of their own: an indexed ring goes to scratch memory, which made the loop four
-// times slower) and two in LDS.
+// times slower) and two in LDS.  The smallest tile, which is taken where there are few, has four groups of waves that take
+// every fourth step each and add their sums at the end (a bf16 1024 x 4096: 392 us with one group, 382 with two, 368 with
+// four; two groups for the middle tile: 4.91 instead of 4.65 ms for fp32 4096 x 4096).
 template <int BM_> struct Cfg {
   static constexpr int BM = BM_, BK = 32;
-  static constexpr int THREADS = BM == 256 ? 512 : 256;
-  static constexpr int AHEAD = BM == 64 ? 4 : BM == 128 ? 2 : 1;
+  static constexpr int WAVES = BM == 256 ? 8 : 4;  // that share a step
+  static constexpr int GROUPS = BM == 64 ? 4 : 1;  // of them, that take the steps in turn
+  static constexpr int THREADS = GROUPS * WAVES * 64;
+  static constexpr int AHEAD = BM == 256 ? 1 : 2;
   static constexpr int WM = BM / (BM == 256 ? 4 : 2), WN = BM / 2;  // a wave's rows and columns
   static constexpr int TM = WM / 32, TN = WN / 32;                  // 32 x 32 blocks of them
   static constexpr int TILE = BM / 64 * 2 * kBlock;                 // halves of an operand's step in LDS
-  static constexpr int NPT = TILE * 2 / 16 / THREADS;               // 16-byte pieces of it per thread
+  static constexpr size_t LDS = (size_t)GROUPS * 4 * TILE * sizeof(_Float16);
+  static constexpr int NPT = TILE * 2 / 16 / (WAVES * 64);          // 16-byte pieces of it per thread
 };
 
 template <int BM, bool SUMS>
 __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g, const Product p) {
   using C = Cfg<BM>;
-  extern __shared__ __attribute__((aligned(16))) _Float16 lds_all[];  // [2][A, B][TILE]
+  extern __shared__ __attribute__((aligned(16))) _Float16 lds_everyone[];  // [GROUPS][2][A, B][TILE]
   const int gi = which(g, blockIdx.x);
   const Mat& mat = g.mats[gi];
   const Layout l = layout_of(mat.rows, mat.cols);
   char* const ws = g.base + mat.ws;
   const int block = blockIdx.x - g.first[gi];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int turns = wave_all / C::WAVES, wave = wave_all % C::WAVES, tid = wave * 64 + lane;
+  _Float16* const lds_all = lds_everyone + turns * 4 * C::TILE;
   const float x0 = *reinterpret_cast<const float*>(ws);
 
   const bool apply = p.shape == SHAPE_APPLY, gram = p.shape == SHAPE_GRAM;
@@ -264,13 +280,13 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
   const _Float16* B = reinterpret_cast<const _Float16*>(ws + (gram ? l.x : apply ? l.xt(p.from) : l.sq(p.b)));
   // (a 128-row tile may reach past an operand, which is padded to 64 rows: it reads the last block again and does not
   // store those results)
-  const int steps = K / C::BK;
+  const int steps = K / C::BK, rounds = (steps + C::GROUPS - 1) / C::GROUPS;
   struct Step { u32x4 a[C::NPT], b[C::NPT]; };
-  auto fetch = [&](Step& r, int step) {
-    step = min(step, steps - 1);
+  auto fetch = [&](Step& r, int round) {
+    const int step = min(round * C::GROUPS + turns, steps - 1);
 #pragma unroll
     for (int i = 0; i < C::NPT; ++i) {
-      const int idx = tid + i * C::THREADS, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;
+      const int idx = tid + i * C::WAVES * 64, sub = idx / (2 * kBlock / 8), in = idx % (2 * kBlock / 8) * 8;
       const int64_t ra = (int64_t)min((i0 >> 6) + sub, (M >> 6) - 1) * (K >> 5) + step;
       const int64_t rb = (int64_t)min((j0 >> 6) + sub, (N >> 6) - 1) * (K >> 5) + step;
       r.a[i] = *reinterpret_cast<const u32x4*>(A + ra * (2 * kBlock) + in);
@@ -280,7 +296,7 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
   auto put = [&](const Step& r, int buf) {
 #pragma unroll
     for (int i = 0; i < C::NPT; ++i) {
-      _Float16* const at = lds_all + buf * 2 * C::TILE + (tid + i * C::THREADS) * 8;
+      _Float16* const at = lds_all + buf * 2 * C::TILE + (tid + i * C::WAVES * 64) * 8;
       *reinterpret_cast<u32x4*>(at) = r.a[i];
       *reinterpret_cast<u32x4*>(at + C::TILE) = r.b[i];
     }
@@ -330,8 +346,9 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
   // SUMS (fp32 in the smallest tile): each step has a sum of its own, as for the small matrices (200 x 1000: 2.4e-6 instead
   // of 4.1e-6 off, by the definition 2.6e-6; 16 bits round coarser than either, and a bf16 1024 x 4096 takes 394 us without
   // and 448 us with it)
-  auto turn = [&](int buf, Step& r, int later) {
-    if constexpr (SUMS) {
+  auto turn = [&](int round, int buf, Step& r, int later) {
+    if (C::GROUPS > 1 && round * C::GROUPS + turns >= steps) {
+    } else if constexpr (SUMS) {
       f32x16 part[C::TM][C::TN];
 #pragma unroll
       for (int i = 0; i < C::TM; ++i)
@@ -353,32 +370,15 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
     fetch(r, later);
     __syncthreads();
   };
-  if constexpr (C::AHEAD == 4) {
-    Step r0, r1, r2, r3;
-    fetch(r0, 0);
-    fetch(r1, 1);
-    fetch(r2, 2);
-    fetch(r3, 3);
-    put(r0, 0);
-    fetch(r0, 4);
-    __syncthreads();
-    for (int s = 0;; s += 4) {
-      turn(0, r1, s + 5);
-      turn(1, r2, s + 6);
-      if (s + 2 >= steps) break;
-      turn(0, r3, s + 7);
-      turn(1, r0, s + 8);
-      if (s + 4 >= steps) break;
-    }
-  } else if constexpr (C::AHEAD == 1) {  // (two would not fit the registers of two waves per SIMD)
+  if constexpr (C::AHEAD == 1) {  // (two would not fit the registers of two waves per SIMD)
     Step r0;
     fetch(r0, 0);
     put(r0, 0);
     fetch(r0, 1);
     __syncthreads();
-    for (int s = 0; s < steps; s += 2) {
-      turn(0, r0, s + 2);
-      turn(1, r0, s + 3);
+    for (int s = 0; s < rounds; s += 2) {
+      turn(s, 0, r0, s + 2);
+      turn(s + 1, 1, r0, s + 3);
     }
   } else {
     Step r0, r1;
@@ -387,10 +387,45 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
     put(r0, 0);
     fetch(r0, 2);
     __syncthreads();
-    for (int s = 0; s < steps; s += 2) {
-      turn(0, r1, s + 3);
-      turn(1, r0, s + 4);
+    for (int s = 0; s < rounds; s += 2) {
+      turn(s, 0, r1, s + 3);
+      turn(s + 1, 1, r0, s + 4);
     }
+  }
+  // The groups' sums, added in their order; each group then finishes its share of every block's rows.
+  constexpr int SHARE = 4 / C::GROUPS;
+  f32x4 sums[C::TM][C::TN][SHARE];
+  if constexpr (C::GROUPS > 1) {
+    f32x4* const all = reinterpret_cast<f32x4*>(lds_everyone) + wave * C::TM * C::TN * 4 * 64 + lane;
+    constexpr int GROUP = C::WAVES * C::TM * C::TN * 4 * 64;
+#pragma unroll
+    for (int bi = 0; bi < C::TM; ++bi)
+#pragma unroll
+      for (int bj = 0; bj < C::TN; ++bj)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4)
+          all[turns * GROUP + ((bi * C::TN + bj) * 4 + e4) * 64] =
+              f32x4{acc[bi][bj][e4 * 4], acc[bi][bj][e4 * 4 + 1], acc[bi][bj][e4 * 4 + 2], acc[bi][bj][e4 * 4 + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int bi = 0; bi < C::TM; ++bi)
+#pragma unroll
+      for (int bj = 0; bj < C::TN; ++bj)
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+          const int at = ((bi * C::TN + bj) * 4 + turns * SHARE + i) * 64;
+          f32x4 v = all[at];
+#pragma unroll
+          for (int q = 1; q < C::GROUPS; ++q) v += all[q * GROUP + at];
+          sums[bi][bj][i] = v;
+        }
+  } else {
+#pragma unroll
+    for (int bi = 0; bi < C::TM; ++bi)
+#pragma unroll
+      for (int bj = 0; bj < C::TN; ++bj)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sums[bi][bj][e / 4][e % 4] = acc[bi][bj][e];
   }
 
   // results: column = lane & 31, rows 8 (e / 4) + 4 (lane >> 5) + e % 4 of a 32 x 32 block
@@ -405,14 +440,15 @@ __global__ __launch_bounds__(Cfg<BM>::THREADS) void product_kernel(const Group g
 #pragma unroll
     for (int bj = 0; bj < C::TN; ++bj)
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
+      for (int share = 0; share < SHARE; ++share) {
+        const int e4 = turns * SHARE + share;
         const int row = i0 + wi + bi * 32 + e4 * 8 + (lane >> 5) * 4, col = j0 + wj + bj * 32 + (lane & 31);
         if (row >= M || col >= N) continue;
         float v[4];
         f16x4 hi, lo;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = acc[bi][bj][e4 * 4 + e] * unscale;
+          v[e] = sums[bi][bj][share][e] * unscale;
           if (!apply) {
             if (R != nullptr) {
               const int64_t at = at_of(row + e, col, l.mp);
@@ -769,11 +805,10 @@ int launch_tiles(Group& g, const Product& p, hipStream_t stream) {
     blocks += tiles_of(g.mats[i], p.shape, BM);
     HIVT_REQUIRE(blocks < ((int64_t)1 << 31), HIVT_ERR_ARG, "%s: too many workgroups", what);
   }
-  const size_t lds = (size_t)4 * C::TILE * sizeof(_Float16);
-  if (lds > 48 * 1024)
+  if (C::LDS > 48 * 1024)
     HIVT_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<BM, SUMS>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), what);
-  hipLaunchKernelGGL((product_kernel<BM, SUMS>), dim3((unsigned)blocks), dim3(C::THREADS), lds, stream, g, p);
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS), what);
+  hipLaunchKernelGGL((product_kernel<BM, SUMS>), dim3((unsigned)blocks), dim3(C::THREADS), C::LDS, stream, g, p);
   HIVT_CHECK_LAUNCH(what);
   return HIVT_OK;
 }

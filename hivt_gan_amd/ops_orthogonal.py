@@ -71,9 +71,10 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = 5, eps: float =
     """Each matrix [rows, cols] of the list, its singular values brought near 1: ``x / (|x| + eps)`` (Frobenius norm), then
     ``steps`` times ``x <- a x + (b g + c g^2) x`` with g = x x^T (of the shorter side) and a, b, c = 3.4445, -4.7750,
     2.0315.  One type for the list, float32, bfloat16 or float16; any shapes up to 65536 a side.  The arithmetic is that of
-    fp32 whatever the type, rounded once at the end; results are the same whatever else is in the list.  ``out``:
-    contiguous tensors to write to (each may be its own matrix, and shares no memory with any other one or output); without
-    it, results of one shape are slices of one allocation.  Not differentiable."""
+    fp32 whatever the type, rounded once at the end; equal calls give equal bits, and what else is in the list moves a
+    result by the rounding of fp32 sums at most.  ``out``: contiguous tensors to write to (each may be its own matrix, and
+    shares no memory with any other one or output); without it, results of one shape are slices of one allocation.  Not
+    differentiable."""
     matrices = list(matrices)
     if not matrices:
         return []

@@ -609,9 +609,9 @@ int hivt_qk_norm_rotary_bwd(const hivt_qk_norm_rotary* p, const double* rates, f
  *
  *   X = in / (|in| + eps) (Frobenius norm), then `steps` times X <- a X + (b G + c G^2) X, G = X X' (X' X for a matrix
  *   with more rows than columns), with a, b, c = 3.4445, -4.7750, 2.0315: the singular values go near 1.  out = X.
- * in and out are contiguous row-major matrices of one type; in == out of
- * one entry is allowed; an output shares memory with no other entry.  The host array is read before the
- * call returns.  Results are accurate to fp32 (see the kernels) and do not depend on what else is in the list.
+ * in and out are contiguous row-major matrices of one type; in == out of one entry is allowed, and an output shares
+ * memory with no other entry.  The host array is read before the call returns.  Results are accurate to fp32 (see the
+ * kernels); what else is in the list may change the order of a sum, nothing more.
  * ------------------------------------------------------------------------------------------ */
 typedef struct {
   int64_t in, out;    /* device addresses */
