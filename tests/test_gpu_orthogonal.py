@@ -186,3 +186,10 @@ def test_outputs_that_share_memory():
     got = ops.orthogonalize([a, b], out=[a, c])
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a, want[0])
     assert store._version > version
+
+
+def test_tiles_left_for_a_last_turn():
+    """32 lists of 128-row tiles: 528 of them on and below the diagonal, and 12 x 45 of a product with X."""
+    for rows, cols in ((4000, 4100), (1500, 5700)):
+        x = gaussian(rows, cols)
+        check(ops.orthogonalize([x], steps=2)[0], x, steps=2, tol=1e-5)
