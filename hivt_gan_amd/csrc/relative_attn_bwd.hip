@@ -28,14 +28,27 @@ __device__ __forceinline__ float dot(const Frag<T, E>& a, const Frag<T, E>& b) {
 }
 
 // Waves to a SIMD: two where the registers allow, so that one's matrix instructions run beside the other's exponentials.
+// Bound by issue and latency, as the forward: bf16 2 x 4096 causal, 16 heads of 128: 359 us, 575 TFLOP/s; 8 x 1024, 16
+// heads of 64: 88 us, 585 TFLOP/s; fp32 64 x 301, 8 heads of 16: 75 us.
+// The widest 16-bit heads need two LDS buffers for that (`paired`): keys are on their way to the other one during the
+// first half of a tile and values during the second, in the same registers (505 -> 359 us).
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2) : DP <= (sizeof(T) == 4 ? 32 : 96) ? 2 : 1) void dq_kernel(const Args a, float2* __restrict__ far_sums) {
+__host__ __device__ constexpr bool paired() { return sizeof(T) == 2 && DP > 96 && QB == 2; }
+template <typename T, int DP, int QB>
+__host__ __device__ constexpr int waves_per_simd() {
+  if (sizeof(T) == 2) return 2;
+  return QB == 1 ? (DP >= 128 ? 1 : 2) : DP <= 32 ? 2 : 1;
+}
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256, (waves_per_simd<T, DP, QB>())) void dq_kernel(const Args a, float2* __restrict__ far_sums) {
   using TL = Tile<T, DP>;
   constexpr int NB = DP / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const kt = reinterpret_cast<T*>(smem);
   T* const vt = kt + kBN * TL::PITCH;
-  float* const bias = reinterpret_cast<float*>(vt + kBN * TL::PITCH);
+  constexpr bool PAIRED = paired<T, DP, QB>();
+  constexpr int BUFFER = 2 * kBN * TL::PITCH;
+  float* const bias = reinterpret_cast<float*>(kt + (PAIRED ? 2 : 1) * BUFFER);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
   const int qtiles = (a.M + 64 * QB - 1) / (64 * QB);
@@ -91,108 +104,143 @@ __global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2
 
   const T* const kbase = static_cast<const T*>(a.k) + b * a.k_st[0] + g * a.k_st[2];
   const T* const vbase = static_cast<const T*>(a.v) + b * a.v_st[0] + g * a.v_st[2];
-  Loader<T, DP, kBN, 256> kl, vl;
-  uint64_t bits = 0;
-  int t = 0;
-  auto seek = [&]() {
-    while (t < t_end && (bits = tile_keys(a, b, t * kBN, lane)) == 0) ++t;
-    if (t < t_end) {
-      const int64_t k0 = (int64_t)t * kBN;
-      auto keep = [&](int row) { return (bits >> row & 1) != 0; };
-      kl.load(kbase + k0 * a.k_st[1], a.k_st[1], a.d, a.k_align, tid, bits == ~0ull, keep);
-      vl.load(vbase + k0 * a.v_st[1], a.v_st[1], a.d, a.v_align, tid, bits == ~0ull, keep);
-    }
-  };
-  seek();
-  while (t < t_end) {
-    __syncthreads();
-    kl.store(kt, tid);
-    vl.store(vt, tid);
-    const int k0 = t * kBN;
-    const uint64_t keys = bits;
-    ++t;
-    seek();
-    __syncthreads();
-    if (!active || (a.causal && k0 > pos_hi)) continue;
-
+  // half a tile: two 16-key blocks, what the reduction over the keys takes
+  int k0 = 0;
+  uint64_t keys = 0;
+  auto half = [&](int kk, const T* kt, const T* vt) __attribute__((always_inline)) {
+    if (!active || (a.causal && k0 > pos_hi)) return;
     const int rel_hi = k0 + kBN - 1 - pos_lo, rel_lo = k0 - pos_hi;
     const bool left = rel_hi <= -a.sat, right = rel_lo >= hi, far = left || right;
     const bool whole = keys == ~0ull && (!a.causal || rel_hi <= 0);
     const float c = bias[left ? 0 : width - 1];
     const bool plain = far && whole && fabsf(c) <= kPlainBias;  // (see the forward)
-    // two 16-key blocks at a time: what the reduction over the keys takes
+    f32x4 s[2][QB], dp[2][QB];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      f32x4 s[2][QB], dp[2][QB];
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int qb = 0; qb < QB; ++qb) s[i][qb] = dp[i][qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) s[i][qb] = dp[i][qb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int ks = 0; ks < TL::KSTEPS; ++ks) {
+        const Frag<T, TL::E> kf = TL::rows(kt, (2 * kk + i) * 16, ks, lane), vf = TL::rows(vt, (2 * kk + i) * 16, ks, lane);
 #pragma unroll
-        for (int ks = 0; ks < TL::KSTEPS; ++ks) {
-          const Frag<T, TL::E> kf = TL::rows(kt, (2 * kk + i) * 16, ks, lane), vf = TL::rows(vt, (2 * kk + i) * 16, ks, lane);
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) {
-            Frag<T, TL::E>::mma(kf, qf[qb][ks], s[i][qb]);
-            Frag<T, TL::E>::mma(vf, of[qb][ks], dp[i][qb]);
-          }
+        for (int qb = 0; qb < QB; ++qb) {
+          Frag<T, TL::E>::mma(kf, qf[qb][ks], s[i][qb]);
+          Frag<T, TL::E>::mma(vf, of[qb][ks], dp[i][qb]);
         }
       }
-      Frag<T, 8> df[QB];
+    }
+    Frag<T, 8> df[QB];
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        float mul = a.scale2, add = c;  // (see the forward)
-        if (!plain) {
-          if (far) {
+    for (int qb = 0; qb < QB; ++qb) {
+      float mul = a.scale2, add = c;  // (see the forward)
+      if (!plain) {
+        if (far) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, c);
-          } else {
-            const float* const at = bias + k0 + kk * 32 + quad * 4 - pos[qb] + a.sat + kMargin;
+            for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, c);
+        } else {
+          const float* const at = bias + k0 + kk * 32 + quad * 4 - pos[qb] + a.sat + kMargin;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, at[i * 16 + r]);
-          }
-          mul = 1.0f;
-          add = 0.0f;
-          if (!whole) {
-            const int lim = a.causal ? pos[qb] - k0 : kBN;
+            for (int r = 0; r < 4; ++r) s[i][qb][r] = fmaf(s[i][qb][r], a.scale2, at[i * 16 + r]);
+        }
+        mul = 1.0f;
+        add = 0.0f;
+        if (!whole) {
+          const int lim = a.causal ? pos[qb] - k0 : kBN;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t nibble = (uint32_t)(keys >> (kk * 32 + i * 16 + quad * 4));
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const bool out = !(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim;
-                s[i][qb][r] = out ? -INFINITY : s[i][qb][r];
-                dp[i][qb][r] = out ? 0.0f : dp[i][qb][r];
-              }
+            for (int r = 0; r < 4; ++r) {
+              const bool out = !(nibble >> r & 1) || kk * 32 + i * 16 + quad * 4 + r > lim;
+              s[i][qb][r] = out ? -INFINITY : s[i][qb][r];
+              dp[i][qb][r] = out ? 0.0f : dp[i][qb][r];
             }
           }
         }
-        const float shift = add - m[qb];
-        float sum_ds = 0.0f, sum_p = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float p = fexp2(fmaf(s[i][qb][r], mul, shift)) * il[qb];
-            dp[i][qb][r] = p * (dp[i][qb][r] - delta[qb]);
-            sum_ds += dp[i][qb][r];
-            sum_p += p;
-          }
-        rsum[qb] += sum_ds;
-        if (left) { far_l[qb] += sum_ds; w_l[qb] += sum_p; }
-        else if (right) { far_r[qb] += sum_ds; w_r[qb] += sum_p; }
-        df[qb] = pair_frag<T>(dp[0][qb], dp[1][qb]);
       }
+      const float shift = add - m[qb];
+      float sum_ds = 0.0f, sum_p = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const Frag<T, 8> kf = TL::cols(kt, kk * 32, n * 16, lane);
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) Frag<T, 8>::mma(kf, df[qb], dq[n][qb]);
+        for (int r = 0; r < 4; ++r) {
+          const float p = fexp2(fmaf(s[i][qb][r], mul, shift)) * il[qb];
+          dp[i][qb][r] = p * (dp[i][qb][r] - delta[qb]);
+          sum_ds += dp[i][qb][r];
+          sum_p += p;
+        }
+      rsum[qb] += sum_ds;
+      if (left) { far_l[qb] += sum_ds; w_l[qb] += sum_p; }
+      else if (right) { far_r[qb] += sum_ds; w_r[qb] += sum_p; }
+      df[qb] = pair_frag<T>(dp[0][qb], dp[1][qb]);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const Frag<T, 8> kf = TL::cols(kt, kk * 32, n * 16, lane);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) Frag<T, 8>::mma(kf, df[qb], dq[n][qb]);
+    }
+  };
+
+  int t = 0;
+  uint64_t bits = 0;
+  auto seek = [&]() {  // to the next tile that holds an allowed key
+    while (t < t_end && (bits = tile_keys(a, b, t * kBN, lane)) == 0) ++t;
+  };
+  Loader<T, DP, kBN, 256> kl, vl;
+  auto load = [&](Loader<T, DP, kBN, 256>& l, const T* base, const int64_t* st, int align) {
+    auto keep = [&](int row) { return (bits >> row & 1) != 0; };
+    l.load(base + (int64_t)t * kBN * st[1], st[1], a.d, align, tid, bits == ~0ull, keep);
+  };
+  seek();
+  if constexpr (PAIRED) {
+    int at = 0;
+    if (t < t_end) {
+      load(kl, kbase, a.k_st, a.k_align);
+      load(vl, vbase, a.v_st, a.v_align);
+      kl.store(kt, tid);
+      vl.store(vt, tid);
+    }
+    while (t < t_end) {
+      __syncthreads();  // this buffer has been filled, the other one read by every wave
+      k0 = t * kBN;
+      keys = bits;
+      ++t;
+      seek();
+      if (t < t_end) load(kl, kbase, a.k_st, a.k_align);
+      half(0, kt + at, vt + at);
+      if (t < t_end) {
+        kl.store(kt + (BUFFER - at), tid);
+        load(kl, vbase, a.v_st, a.v_align);
       }
+      half(1, kt + at, vt + at);
+      if (t < t_end) kl.store(vt + (BUFFER - at), tid);
+      at = BUFFER - at;
+    }
+  } else {
+    if (t < t_end) {
+      load(kl, kbase, a.k_st, a.k_align);
+      load(vl, vbase, a.v_st, a.v_align);
+    }
+    while (t < t_end) {
+      __syncthreads();
+      kl.store(kt, tid);
+      vl.store(vt, tid);
+      k0 = t * kBN;
+      keys = bits;
+      ++t;
+      seek();
+      if (t < t_end) {
+        load(kl, kbase, a.k_st, a.k_align);
+        load(vl, vbase, a.v_st, a.v_align);
+      }
+      __syncthreads();
+      half(0, kt, vt);
+      half(1, kt, vt);
     }
   }
   if (!active) return;
@@ -223,7 +271,8 @@ __global__ __launch_bounds__(256, QB == 1 ? (sizeof(T) == 4 && DP >= 128 ? 1 : 2
   }
 }
 
-// BQ query rows a step; a wave owns 16 KB keys, a workgroup has WAVES of them.
+// BQ query rows a step; a wave owns 16 KB keys, a workgroup has WAVES of them.  Four products to dq_kernel's three, bound
+// by the same; in the order of its cases: 529 us, 520 TFLOP/s; 124 us, 554 TFLOP/s; 92 us.
 template <typename T, int DP, int KB, int BQ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(const Args a) {
   using TL = Tile<T, DP>;
@@ -414,7 +463,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(con
   }
 }
 
-// dk, dv = the sums of the query heads' shares, in ascending order of the heads
+// dk, dv = the sums of the query heads' shares, in ascending order of the heads; bound by memory (2 x 4096, 4 of 16 heads
+// of 128: 151 MB in 43 us, 3.5 TB/s)
 template <typename T>
 __global__ __launch_bounds__(256) void group_kernel(const Args a) {
   const int64_t rows = (int64_t)a.B * a.N * a.G, total = rows * 2 * a.d;
@@ -431,7 +481,8 @@ __global__ __launch_bounds__(256) void group_kernel(const Args a) {
 
 // Sums of ds over the buckets, for 16 QB query rows of one (batch, head): the tiles that dq_kernel did not count as far.
 // The tile of ds passes through LDS so that a lane can add along a diagonal; diagonals add up in LDS (one lane each, no
-// conflicts), distances beyond the last border in registers.
+// conflicts), distances beyond the last border in registers.  A chain of small products, LDS and waits, one wave to a tile:
+// 86, 58 and 50 us in the cases of dq_kernel.
 template <typename T, int DP, int QB>
 __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __restrict__ far_sums,
                                                   float* __restrict__ partial) {
@@ -569,7 +620,7 @@ __global__ __launch_bounds__(64) void bias_kernel(const Args a, const float2* __
 }
 
 // d_table[bucket][h] = sum over the rows of partial [rows][H][buckets]: a workgroup takes 64 columns and cuts the rows into
-// 16 slices, each added in ascending order, then the slices; in 64 bits.
+// 16 slices, each added in ascending order, then the slices; in 64 bits.  5 us, its launch.
 __global__ __launch_bounds__(1024) void table_kernel(const float* __restrict__ partial, int64_t rows, int H, int buckets,
                                                      float* __restrict__ d_table) {
   __shared__ double sums[16][64];
@@ -644,7 +695,7 @@ int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
   const size_t table = (size_t)bias_width(a) * sizeof(float);
   float2* const far_sums = a.want_table ? reinterpret_cast<float2*>(ws + w.far) : nullptr;
   const int64_t blocks = (int64_t)a.B * a.H * ((a.M + 64 * QB - 1) / (64 * QB));
-  const size_t lds = (size_t)2 * kBN * TL::PITCH * sizeof(T) + table;
+  const size_t lds = (size_t)(paired<T, DP, QB>() ? 4 : 2) * kBN * TL::PITCH * sizeof(T) + table;
   HIVT_REQUIRE(blocks < ((int64_t)1 << 31) && (int64_t)a.B * a.H * w.groups < ((int64_t)1 << 31), HIVT_ERR_ARG,
                "%s: too many workgroups", what);
   if (lds > 48 * 1024)
