@@ -272,7 +272,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, DP, QB>())) void dq_kernel(
 }
 
 // BQ query rows a step; a wave owns 16 KB keys, a workgroup has WAVES of them.  Four products to dq_kernel's three, bound
-// by the same; in the order of its cases: 529 us, 520 TFLOP/s; 124 us, 554 TFLOP/s; 92 us.
+// by the same; in the order of its cases: 475 us, 579 TFLOP/s; 124 us, 554 TFLOP/s; 92 us.  (Two LDS buffers, as in
+// dq_kernel, cost registers and gained nothing here: 1.18 -> 1.20 ms for the whole of the first case.)
 template <typename T, int DP, int KB, int BQ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 2 : 1) void dkv_kernel(const Args a) {
   using TL = Tile<T, DP>;
@@ -720,10 +721,12 @@ int launch_rows(const Args& a, char* ws, const Work& w, hipStream_t stream) {
 template <typename T, int DP>
 int launch_width(const Args& a, char* ws, const Work& w, hipStream_t stream) {
   using TL = Tile<T, DP>;
-  // 32 keys to a wave where its operands and sums fit the registers (fp32 at 96 wide and more: they do not).  A narrow
-  // head leaves room for two waves per SIMD; a wide one gets workgroups of two waves: two of them share a compute unit,
-  // and twice as many of half the length even out the causal ones (decoder layer of 4096 positions, with a query head to a workgroup: 1350 -> 523 us).
-  constexpr int KB = sizeof(T) == 4 && DP >= 96 ? 1 : 2, BQ = 32, WAVES = DP <= (sizeof(T) == 4 ? 32 : 64) ? 4 : 2;
+  // 32 keys to a wave where that leaves two waves per SIMD, 16 for the widest heads (bf16, decoder layer of 4096 positions:
+  // 32 keys in workgroups of two waves, one to a SIMD, 529 us, 16 keys in workgroups of four 475 us).  fp32 from 64 wide on
+  // has one wave per SIMD either way; its workgroups are of two waves: two of them share a compute unit, and twice as many
+  // of half the length even out the causal ones.
+  constexpr bool FP32 = sizeof(T) == 4;
+  constexpr int KB = DP >= 96 ? 1 : 2, BQ = 32, WAVES = FP32 && DP > 32 ? 2 : 4;
   const char* what = "hivt_relative_attn_bwd";
   const int rc = rows_per_group(a.M) == 16 ? launch_rows<T, DP, 1>(a, ws, w, stream) : launch_rows<T, DP, 2>(a, ws, w, stream);
   if (rc != HIVT_OK || a.N == 0) return rc;
