@@ -1,7 +1,7 @@
 // Short sequences: one wave to a (batch, head).  Forward: at most 64 queries and 32 keys, or 64 keys with heads of at most
 // 32.  Backward: at most 32 queries and keys, heads of at most 64 (more does not fit the registers twice).
 //
-// At 21 positions with heads of 16 the pass is bound by memory (220 MB forward and backward for 2560 sequences of 8 heads)
+// At 21 positions with heads of 16 the pass is bound by memory (300 MB forward and backward for 2560 sequences of 8 heads)
 // and the general kernels' tiles of 64 keys and 64 rows are mostly padding.  Here every score of a (batch, head) fits the
 // registers of one wave: operands come straight from memory in the lanes' layout (64-byte rows of neighbouring heads,
 // taken by neighbouring waves, share cache lines), there is no LDS tile and no barrier.
