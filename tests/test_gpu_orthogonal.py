@@ -193,3 +193,12 @@ def test_tiles_left_for_a_last_turn():
     for rows, cols in ((4000, 4100), (1500, 5700)):
         x = gaussian(rows, cols)
         check(ops.orthogonalize([x], steps=2)[0], x, steps=2, tol=1e-5)
+
+
+def test_tiles_left_in_16_bits_and_in_lists():
+    x = gaussian(4000, 4100, torch.bfloat16)
+    check(ops.orthogonalize([x], steps=1)[0], x, steps=1)
+    xs = [gaussian(900, 1000, torch.float16, seed=i, scale=1.0) for i in range(15)]  # 540 tiles, the last 28 in quarters
+    ys = ops.orthogonalize(xs, steps=2)
+    for i in (0, 13, 14):
+        check(ys[i], xs[i], steps=2)

@@ -373,6 +373,30 @@ def test_without_gradients_equal_bits():
     assert not got.requires_grad and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,H,G,d,buckets,distance,causal", [
+    (200, 333, 4, 2, 128, 32, 4096, True), (131, 131, 2, 1, 97, 32, 20, False), (70, 700, 3, 3, 100, 16, 300, False),
+    (257, 190, 2, 2, 127, 8, 16, True), (1, 500, 16, 1, 128, 32, 4096, True), (33, 65, 8, 1, 81, 32, 4096, False)])
+def test_wide_heads(dtype, M, N, H, G, d, buckets, distance, causal):
+    """Heads from 81 on, masked in runs (whole tiles too) and one by one, with the longest tables and odd strides."""
+    q, k, v, table, o = inputs(2, M, N, H, G, d, dtype, buckets)
+    mask = torch.rand(2, N, generator=torch.Generator().manual_seed(3)) < 0.3
+    mask[0, 64:192] = True
+    mask[1, :70] = True
+    check(q, k, v, table, o, causal, max_distance=distance, mask=mask.to(DEV))
+    wide = torch.zeros(2, N, G, 2 * d + 3, dtype=dtype, device=DEV)
+    wide[..., 1:d + 1], wide[..., d + 2:2 * d + 2] = k, v
+    check(q, wide[..., 1:d + 1], wide[..., d + 2:2 * d + 2], table, o[:, :, :1].expand(2, M, H, d), causal,
+          max_distance=distance)
+
+
+def test_broadcast_inputs():
+    """Tensors whose strides are zero: one sequence of keys for the batch, one query row, one gradient."""
+    q, k, v, table, o = inputs(3, 80, 90, 4, 2, 16, torch.float32, 8)
+    check(q[:1, :1].expand(3, 80, 4, 16), k[:1].expand(3, 90, 2, 16), v[:, :1].expand(3, 90, 2, 16), table,
+          o[:1, :1, :1, :1].expand(3, 80, 4, 16), True)
+
+
 def test_refusals():
     q, k, v, table, o = inputs(1, 8, 8, 4, 2, 16, torch.float32, 8)
     call = ops.relative_attention
